@@ -1454,7 +1454,7 @@ hipError_t launch_qk_rope_store(const PageGeom& g, const RopeGeom& r, const int3
   // tile layout's widths stop at 256, so VPL is 1, 2 or 4.
   const uint32_t vpl = g.hd / 64, half = r.half_rot;
   const bool neox = (r.flags & ROPE_NEOX) != 0;
-  const bool pairs_ok = half == 0 || !neox || (half % vpl == 0 && ((half / vpl) & (half / vpl - 1)) == 0);
+  const bool pairs_ok = half == 0 || !neox || (vpl != 0 && half % vpl == 0 && ((half / vpl) & (half / vpl - 1)) == 0);
   const bool reg = g.layout == LAYOUT_TILES && g.hd == g.hdv && g.hd % 64 == 0 &&
                    (vpl == 1 || vpl == 2 || vpl == 4) && pairs_ok;
   if (reg) {
