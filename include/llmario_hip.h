@@ -235,6 +235,30 @@ int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint6
                           const float* q_in, const float* k_in, const float* v_in, float* q_out,
                           const lmh_rope_params* params, void* stream);
 
+/* lmh_qk_rope_store at positions of several axes (the time, height and width of an image's or a video's patches;
+ * the reference rotates by the sequence position alone): pair i of row t turns by
+ *   positions[axis(i)][t] * freq_scale * theta^(-2i/rot_dim)  (/ freq_div[i]),
+ * computed in 64 bits (lmh_qk_rope_store forms its angles in f32, as the reference does; the two agree to that
+ * rounding where every axis holds the sequence position). The row is stored at its sequence position, which the
+ * segments give, as ever. axis(i): the pairs of axis 0, then axis 1, .. (sections[a] pairs each, summing to
+ * rot_dim / 2); with LMH_ROPE_AXES_INTERLEAVED the axes take turns, a = i mod n_axes, axes from 1 on for
+ * sections[a] turns (a + n_axes * (sections[a] - 1) < rot_dim / 2) and axis 0 every other pair. With
+ * LMH_ROPE_AXES_OWN_FREQ each axis has frequencies of its own: pair j of its n pairs has theta^(-j/n). Everything
+ * else as lmh_qk_rope_store, whose flags must hold LMH_ROPE_APPLY. */
+#define LMH_ROPE_AXES_INTERLEAVED 1u
+#define LMH_ROPE_AXES_OWN_FREQ 2u
+typedef struct lmh_rope_axes {
+  uint32_t abi_version;      /* LMH_ABI_VERSION */
+  uint32_t n_axes;           /* 1 .. 4 */
+  uint32_t flags;            /* LMH_ROPE_AXES_* */
+  uint32_t sections[4];      /* pairs of each axis; 0 past n_axes */
+  uint32_t reserved0;        /* 0 */
+  const int32_t* positions;  /* device [n_axes][n_rows] */
+} lmh_rope_axes;
+int32_t lmh_qk_rope_store_axes(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs,
+                               const float* q_in, const float* k_in, const float* v_in, float* q_out,
+                               const lmh_rope_params* params, const lmh_rope_axes* axes, void* stream);
+
 /* attend (forward.rs:585-678) + attend_split (forward.rs:688-807) in one call: every row t of
  * the segments (sequence segs[i].seq, position pos0+j) attends causally to positions
  * p_lo..=pos of its own sequence (p_lo = pos+1-window when window > 0 and pos+1 > window, else 0),
@@ -268,6 +292,37 @@ int32_t lmh_attend(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_s
  * timing hook records nothing for these calls. */
 int32_t lmh_attend_noalloc(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs,
                            const float* q, float* out, float scale, uint64_t window, void* stream);
+
+/* lmh_attend with shaped scores and a range of keys for each row (the reference's attention is causal with
+ * unshaped scores: forward.rs:585-678). With s = scale * q.K of a row at position pos and a key at position k:
+ *   cap > 0:  s = cap * tanh(s / cap);
+ *   slopes:   s = s - slopes[head] * |pos - k|, after the cap (slopes: device, [n_head] f32);
+ * the row sees keys row_lo[t] <= k < row_hi[t], and with a window only k > pos - window. row_lo / row_hi are host
+ * arrays of one value per row t of the stacked batch, read before the call returns (NULL: 0 / pos + 1). A document
+ * mask is row_lo = the row's document's first position; a prefix mask, or a span whose tokens see each other,
+ * row_hi = the span's end for the rows inside it. A key past the row's own position must be one of the row's
+ * segment (row_hi <= pos0 + n, LMH_INVALID_ARGUMENT otherwise): store the segment's rows first. row_lo >= row_hi,
+ * or a window that leaves nothing: the row sees no key and its output is zeros. out = softmax(s) V over the keys
+ * it sees; what any other key holds does not matter (NaN and infinities included), a K or V that is not finite
+ * and is seen leaves the outputs of the rows that see it not finite or undefined. Scores, softmax and sums are
+ * held in f32, Q and the weights to 22 bits or more. Layers, segments, q, out, stream and errors as lmh_attend's
+ * (window layers: window is 1 .. the layer's width); every geometry is accepted. f16 / bf16 / f32 pages and q8_0
+ * tiles run on matrix cores as one launch (and a merge launch where few rows see many keys), q8_0 rows off the
+ * tiles, widths off a multiple of 8 (f32: 4) or over 256 and blocks under 16 positions on a slower kernel. The
+ * split settings of lmh_attend_tuning do not apply, except prefill_whole_units. A stream under graph capture is
+ * refused with LMH_UNSUPPORTED, as by lmh_attend. */
+typedef struct lmh_score_params {
+  uint32_t abi_version;     /* LMH_ABI_VERSION */
+  uint32_t reserved0;       /* 0 */
+  float scale;
+  float cap;                /* 0: none */
+  const float* slopes;      /* device [n_head], or NULL: no distance bias */
+  const uint32_t* row_lo;   /* host [n_rows], or NULL */
+  const uint32_t* row_hi;   /* host [n_rows], or NULL */
+  uint64_t window;          /* 0: none */
+} lmh_score_params;
+int32_t lmh_attend_scored(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q,
+                          float* out, const lmh_score_params* params, void* stream);
 
 /* Handle options of lmh_attend's planning and precision (no counterpart in the reference, whose
  * CPU path has no such choices; its thread-count split rule is forward.rs:613-633). Set once or
@@ -377,6 +432,12 @@ typedef struct lmh_plan_wave_counts {
 int32_t lmh_plan_unit_waves(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, uint32_t waves_per_cu,
                             uint32_t* waves, uint64_t waves_cap, uint32_t* merges, uint64_t merges_cap,
                             lmh_plan_wave_counts* counts);
+/* The same for lmh_attend_scored, whose rows see keys row_lo[t] .. row_hi[t] - 1 (either NULL, as there): the wave
+ * records of its unit launch, or the decode items of a geometry without one, eight words each, and the merges. */
+int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, const uint32_t* row_lo,
+                        const uint32_t* row_hi, uint32_t waves_per_cu, uint32_t* waves, uint64_t waves_cap,
+                        uint32_t* items, uint64_t items_cap, uint32_t* merges, uint64_t merges_cap,
+                        lmh_plan_wave_counts* counts, uint64_t* n_items);
 
 /* ---- request scheduler: the host side of the batch hand-off ----
  * Scheduler (crates/engine/sched/src/lib.rs:75-282) over the block pool, with Sequence

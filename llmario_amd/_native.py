@@ -59,6 +59,19 @@ class RopeParams(C.Structure):
                 ("attn_factor", C.c_float), ("q_norm", P), ("k_norm", P), ("freq_div", P)]
 
 
+ROPE_AXES_INTERLEAVED, ROPE_AXES_OWN_FREQ = 1, 2
+
+
+class RopeAxes(C.Structure):
+    _fields_ = [("abi_version", u32), ("n_axes", u32), ("flags", u32), ("sections", u32 * 4), ("reserved0", u32),
+                ("positions", P)]
+
+
+class ScoreParams(C.Structure):
+    _fields_ = [("abi_version", u32), ("reserved0", u32), ("scale", C.c_float), ("cap", C.c_float), ("slopes", P),
+                ("row_lo", P), ("row_hi", P), ("window", u64)]
+
+
 class AttendTuning(C.Structure):
     _fields_ = [("abi_version", u32), ("prefill_p_f16", u32), ("prefill_min_rows", u64),
                 ("decode_target_items", u64), ("decode_min_tiles", u64), ("prefill_workgroups", u64),
@@ -160,11 +173,15 @@ SIGNATURES = {
     "lmh_kv_gather": (i32, [P, u32, P, u64, P, P, P]),
     "lmh_kv_gather_encoded": (i32, [P, u32, P, u64, P, P, P]),
     "lmh_qk_rope_store": (i32, [P, u32, P, u64, P, P, P, P, C.POINTER(RopeParams), P]),
+    "lmh_qk_rope_store_axes": (i32, [P, u32, P, u64, P, P, P, P, C.POINTER(RopeParams), C.POINTER(RopeAxes), P]),
     "lmh_attend": (i32, [P, u32, P, u64, P, P, C.c_float, u64, P]),
     "lmh_attend_noalloc": (i32, [P, u32, P, u64, P, P, C.c_float, u64, P]),
+    "lmh_attend_scored": (i32, [P, u32, P, u64, P, P, C.POINTER(ScoreParams), P]),
     "lmh_kv_set_tuning": (i32, [P, C.POINTER(AttendTuning)]),
     "lmh_kv_get_tuning": (i32, [P, C.POINTER(AttendTuning)]),
     "lmh_plan_unit_waves": (i32, [C.POINTER(PlanDesc), P, u64, u32, P, u64, P, u64, C.POINTER(PlanWaveCounts)]),
+    "lmh_plan_scored": (i32, [C.POINTER(PlanDesc), P, u64, P, P, u32, P, u64, P, u64, P, u64, C.POINTER(PlanWaveCounts),
+                              C.POINTER(u64)]),
     "lmh_plan_attend": (i32, [C.POINTER(PlanDesc), P, u64, P, u64, P, u64, P, u64, C.POINTER(PlanCounts)]),
     "lmh_kv_set_timing": (i32, [P, i32]),
     "lmh_kv_kernel_time": (i32, [P, u32, C.POINTER(C.c_double), C.POINTER(u64)]),

@@ -504,10 +504,11 @@ __device__ inline float row_elem(const uint8_t* row, uint32_t d) {
   else return (float)(int8_t)row[d];   // q8_0 code (the caller applies the block scale)
 }
 
-template <int KVT>
+// SC: scores shaped by `sc` (the items' key ranges are the rows' own: sc.ranges is not read).
+template <int KVT, bool SC = false>
 __global__ __launch_bounds__(64 * WAVES) void decode_rows_kernel(PageGeom g, RowGeom r, const DecodeItem* items,
                                                                  uint32_t n_items, const float* q, float* out,
-                                                                 float* part, MergeCopy mc) {
+                                                                 float* part, MergeCopy mc, ScoreGeom sc) {
   constexpr uint32_t ES = KVT == KV_F32 ? 4 : KVT == KV_Q8 ? 1 : 2;   // bytes per value (q8_0: code)
   __shared__ float qs[WAVES][RNG][ROWS_MAX_DIM];
   __shared__ float ps[WAVES][RNG][64];
@@ -529,8 +530,11 @@ __global__ __launch_bounds__(64 * WAVES) void decode_rows_kernel(PageGeom g, Row
   const uint32_t bt_mask = (1u << g.bt_shift) - 1u;
   const uint32_t nd = (hdv + 63) / 64;   // V dims per lane in P.V (<= 8)
   float m[RNG], l[RNG], o[RNG][ROWS_MAX_DIM / 64];
+  float slope[RNG];
+  const uint32_t pos = SC ? (uint32_t)r.row_pos[it.row] : 0u;
 #pragma unroll
   for (int h = 0; h < RNG; h++) {
+    slope[h] = SC && sc.slopes && h < (int)nh ? sc.slopes[it.kvh * r.group + it.h0 + h] * 1.4426950408889634f : 0.f;
     m[h] = -INFINITY;
     l[h] = 0.f;
 #pragma unroll
@@ -574,12 +578,17 @@ __global__ __launch_bounds__(64 * WAVES) void decode_rows_kernel(PageGeom g, Row
 #pragma unroll
     for (int h = 0; h < RNG; h++) {
       if (h >= (int)nh) break;
-      const float sc = valid ? s[h] * r.scale_log2 : -INFINITY;
-      float cm = sc;
+      float sv = s[h] * r.scale_log2;
+      if constexpr (SC) {
+        if (sc.cap_log2 > 0.f) sv = sc.cap_log2 * tanhf(sv);
+        if (sc.slopes) sv = fmaf(-slope[h], fabsf((float)(int)(kk - pos)), sv);
+      }
+      sv = valid ? sv : -INFINITY;
+      float cm = sv;
       for (int x = 32; x >= 1; x >>= 1) cm = fmaxf(cm, __shfl_xor(cm, x));
       const float mn = fmaxf(m[h], cm);
       const float alpha = exp2_fast(m[h] - mn);
-      const float p = exp2_fast(sc - mn);
+      const float p = exp2_fast(sv - mn);
       float ssum = p;
       for (int x = 32; x >= 1; x >>= 1) ssum += __shfl_xor(ssum, x);
       l[h] = l[h] * alpha + ssum;
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_rows_kernel(PageGeom g, Row
     if (h >= (int)nh) break;
     if (it.slot == NO_SLOT) {
       float* op = out + ((size_t)it.row * r.n_head + it.kvh * r.group + it.h0 + h) * hdv;
-      const float inv = 1.0f / l[h];
+      const float inv = SC && l[h] == 0.f ? 0.f : 1.0f / l[h];   // 0: it sees no key
 #pragma unroll
       for (int i = 0; i < (int)(ROWS_MAX_DIM / 64); i++)
         if (lane + 64 * i < hdv) op[lane + 64 * i] = o[h][i] * inv;
@@ -703,7 +712,16 @@ hipError_t launch_rows(const PageGeom& g, const RowGeom& r, const DecodeItem* it
                        const float* q, float* out, float* part, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev) {
   if (g.hd > ROWS_MAX_DIM || g.hdv > ROWS_MAX_DIM || r.ng > (uint32_t)RNG) return hipErrorInvalidValue;
   const dim3 grid((n_items + WAVES - 1) / WAVES), block(64 * WAVES);
-  LMH_LAUNCH(ev, (decode_rows_kernel<KVT>), grid, block, 0, s, g, r, items, n_items, q, out, part, mc);
+  LMH_LAUNCH(ev, (decode_rows_kernel<KVT>), grid, block, 0, s, g, r, items, n_items, q, out, part, mc, ScoreGeom{});
+  return hipGetLastError();
+}
+
+template <int KVT>
+hipError_t launch_rows_scored(const PageGeom& g, const RowGeom& r, const ScoreGeom& sc, const DecodeItem* items, uint32_t n_items,
+                              const float* q, float* out, float* part, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev) {
+  if (g.hd > ROWS_MAX_DIM || g.hdv > ROWS_MAX_DIM || r.ng > (uint32_t)RNG) return hipErrorInvalidValue;
+  const dim3 grid((n_items + WAVES - 1) / WAVES), block(64 * WAVES);
+  LMH_LAUNCH(ev, (decode_rows_kernel<KVT, true>), grid, block, 0, s, g, r, items, n_items, q, out, part, mc, sc);
   return hipGetLastError();
 }
 
@@ -834,6 +852,18 @@ bool decode_mfma_local_ok(uint32_t kv_type, uint32_t hd, uint32_t hdv) {
   LMH_MLOK(KV_F16) LMH_MLOK(KV_BF16) LMH_MLOK(KV_Q8)
 #undef LMH_MLOK
   return false;
+}
+
+hipError_t launch_scored_rows(const PageGeom& g, const RowGeom& r, const ScoreGeom& sc, const DecodeItem* items, uint32_t n_items,
+                              const float* q, float* out, float* part, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev) {
+  if (n_items == 0) return hipSuccess;
+  if (g.layout != LAYOUT_ROWS) return hipErrorInvalidValue;
+  switch (g.kv_type) {
+    case KV_F16: return launch_rows_scored<KV_F16>(g, r, sc, items, n_items, q, out, part, mc, s, ev);
+    case KV_BF16: return launch_rows_scored<KV_BF16>(g, r, sc, items, n_items, q, out, part, mc, s, ev);
+    case KV_Q8: return launch_rows_scored<KV_Q8>(g, r, sc, items, n_items, q, out, part, mc, s, ev);
+    default: return launch_rows_scored<KV_F32>(g, r, sc, items, n_items, q, out, part, mc, s, ev);
+  }
 }
 
 hipError_t launch_decode(const PageGeom& g, const RowGeom& r, const DecodeItem* items, uint32_t n_items,

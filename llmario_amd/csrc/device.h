@@ -99,6 +99,15 @@ struct UnitGeom {
   float* part;       // the call's partial slots
 };
 
+// What lmh_attend_scored's launches make of a score s (in the log2 domain): with a cap, the launch's scale_log2 is
+// scale / cap and the score cap_log2 * tanh(s); then less slopes[head] * |position - key|.
+struct ScoreGeom {
+  float cap_log2 = 0.f;            // cap * log2(e); 0: none
+  const float* slopes = nullptr;   // [n_head] or null
+  const uint2* ranges = nullptr;   // [n_rows]: the first and last key a row sees (first > last: none), or null: causal, window
+};
+
+constexpr uint32_t ROPE_MAX_AXES = 4;
 // Fused per-row tail of attention_block (see lmh_qk_rope_store): flags as LMH_ROPE_*.
 struct RopeGeom {
   uint32_t n_head, q_stride, flags, half_rot;  // half_rot: rotated pairs (0 = no rotation)
@@ -107,6 +116,12 @@ struct RopeGeom {
   const float* k_norm;    // [hd] or null
   const float* freq_div;  // [half_rot] or null
   const float* freq;      // [half_rot] theta^(-2i/rot_dim), computed on the host
+  // positions of several axes (lmh_qk_rope_store_axes), else null: [n_axes][n_rows], and the turns of each pair
+  // per position
+  const int32_t* positions = nullptr;
+  const double* turns = nullptr;
+  uint32_t n_rows = 0, n_axes = 0, interleaved = 0;
+  uint32_t sec[ROPE_MAX_AXES] = {};   // pairs of each axis
 };
 // One row (or the first of an aligned run of four) of a fused store, as the host stages it: a kernel
 // that has it needs no further look-up before its loads.
@@ -211,6 +226,13 @@ uint32_t unit_waves(uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout
 uint32_t unit_waves_per_cu(int32_t device, uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout, uint32_t nb);
 hipError_t launch_units(const PageGeom& g, const UnitGeom& u, uint32_t nb, uint32_t w, const UnitWave* waves, uint32_t n_wg,
                         const float* q, float* out, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev = {});
+// The same with shaped scores (scored.hip), and the row layout's decode items of geometries without an instance.
+uint32_t scored_waves(uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout, uint32_t nb);
+uint32_t scored_waves_per_cu(int32_t device, uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout, uint32_t nb);
+hipError_t launch_scored_units(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, uint32_t nb, uint32_t w, const UnitWave* waves,
+                               uint32_t n_wg, const float* q, float* out, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev = {});
+hipError_t launch_scored_rows(const PageGeom& g, const RowGeom& r, const ScoreGeom& sc, const DecodeItem* items, uint32_t n_items,
+                              const float* q, float* out, float* part, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev = {});
 uint32_t prefill_wg_per_cu();     // prefill workgroups a CU holds when their LDS fits (160 KiB / this)
 uint32_t prefill_cols_per_unit();
 // LDS the prefill kernels declare statically, beside prefill_lds_bytes() of dynamic LDS

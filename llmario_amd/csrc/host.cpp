@@ -286,6 +286,7 @@ struct lmh_kv {
   double acc_ms[6] = {0, 0, 0, 0, 0, 0};
   uint64_t launches[6] = {0, 0, 0, 0, 0, 0};
   std::vector<uint8_t> payload;
+  std::vector<KeyRange> ranges;             // lmh_attend_scored: the keys each row sees
   std::vector<lmh_sched*> scheds;           // schedulers bound to this handle
   // ---- lmh_attend planning / precision options (lmh_kv_set_tuning)
   bool prefill_p_f16 = false;
@@ -1362,9 +1363,48 @@ int32_t lmh_kv_gather_encoded(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, u
   return kv_io(kv, layer, segs, n_segs, k, v, stream, 3);
 }
 
-int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
-                          const float* k_in, const float* v_in, float* q_out, const lmh_rope_params* p,
-                          void* stream) {
+// What is wrong with the axes of a call with `half` rotated pairs, or nullptr.
+static const char* axes_error(const lmh_rope_axes* x, const lmh_rope_params* p, uint32_t half) {
+  if (x->abi_version != LMH_ABI_VERSION) return "rope axes: ABI version";
+  if (!(p->flags & LMH_ROPE_APPLY)) return "rope axes: without LMH_ROPE_APPLY";
+  if (x->n_axes < 1 || x->n_axes > ROPE_MAX_AXES) return "rope axes: n_axes must be 1 .. 4";
+  if (x->flags & ~(LMH_ROPE_AXES_INTERLEAVED | LMH_ROPE_AXES_OWN_FREQ)) return "rope axes: unknown flag";
+  if (x->reserved0) return "rope axes: reserved0 must be 0";
+  if (!(p->theta > 0.f) || !std::isfinite(p->theta) || !std::isfinite(p->freq_scale)) return "rope axes: theta must be positive, freq_scale finite";
+  uint64_t sum = 0;
+  for (uint32_t a = 0; a < ROPE_MAX_AXES; a++) {
+    if (a >= x->n_axes && x->sections[a]) return "rope axes: sections past n_axes must be 0";
+    sum += x->sections[a];
+    if ((x->flags & LMH_ROPE_AXES_INTERLEAVED) && a > 0 && a < x->n_axes && x->sections[a] > 0 &&
+        a + (uint64_t)x->n_axes * (x->sections[a] - 1) >= half)
+      return "rope axes: an interleaved section needs pairs past the last";
+  }
+  if (sum != half) return "rope axes: the sections must sum to rot_dim / 2";
+  return nullptr;
+}
+
+// Turns per position of each rotated pair: freq_scale * theta^(-2i / rot_dim) / 2 pi; with frequencies of its own,
+// pair j of an axis of n pairs turns as pair j of a rotation over 2n dims.
+static void axes_turns(const lmh_rope_axes* x, const lmh_rope_params* p, double* turns) {
+  const uint32_t half = p->rot_dim / 2, n = x->n_axes;
+  const bool mixed = (x->flags & LMH_ROPE_AXES_INTERLEAVED) != 0, alone = (x->flags & LMH_ROPE_AXES_OWN_FREQ) != 0;
+  uint32_t seen[ROPE_MAX_AXES] = {}, at = 0;
+  for (uint32_t i = 0; i < half; i++) {
+    uint32_t a = i % n;
+    if (mixed) a = a != 0 && i < n * x->sections[a] ? a : 0;
+    else {
+      while (seen[at] == x->sections[at]) at++;
+      a = at;
+    }
+    const double e = alone ? -(double)seen[a] / x->sections[a] : -2.0 * i / p->rot_dim;
+    seen[a]++;
+    turns[i] = (double)p->freq_scale * std::pow((double)p->theta, e) * 0.15915494309189533577;
+  }
+}
+
+static int32_t rope_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
+                         const float* k_in, const float* v_in, float* q_out, const lmh_rope_params* p,
+                         const lmh_rope_axes* axes, void* stream) {
   if (!kv) return LMH_INVALID_ARGUMENT;
   if (layer >= kv->layers.size()) return kv->fail(LMH_INVALID_ARGUMENT, "layer out of range");
   if (!p || p->abi_version != LMH_ABI_VERSION) return kv->fail(LMH_INVALID_ARGUMENT, "rope params: null or ABI version");
@@ -1376,6 +1416,7 @@ int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint6
     return kv->fail(LMH_INVALID_ARGUMENT, "rot_dim must be even and in [2, hd]");
   const uint32_t q_stride = p->q_stride ? p->q_stride : y.hd;
   if (q_stride < y.hd) return kv->fail(LMH_INVALID_ARGUMENT, "q_stride < hd");
+  if (const char* bad = axes ? axes_error(axes, p, p->rot_dim / 2) : nullptr) return kv->fail(LMH_INVALID_ARGUMENT, bad);
   if (((p->flags & LMH_ROPE_Q_NORM) && !p->q_norm) || ((p->flags & LMH_ROPE_K_NORM) && !p->k_norm))
     return kv->fail(LMH_INVALID_ARGUMENT, "norm flag without weights");
   if (y.hd > ROPE_MAX_DIM || y.hdv != y.hd)
@@ -1388,11 +1429,19 @@ int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint6
   if (rc != LMH_OK) return rc;
   if (n_rows == 0) return LMH_OK;
   if (!q_in || !k_in || !v_in || !q_out) return kv->fail(LMH_INVALID_ARGUMENT, "null data pointer");
+  if (axes && (!axes->positions || (uintptr_t)axes->positions % 4))
+    return kv->fail(LMH_INVALID_ARGUMENT, "rope axes: null or unaligned positions");
   // rope's per-pair frequency, as the reference forms it in f32 (ops.rs:52):
   // theta.powf(-(2i as f32) / rot_dim as f32)
   const uint32_t half_rot = apply ? p->rot_dim / 2 : 0;
-  std::vector<float> freq(std::max<uint32_t>(half_rot, 1), 0.f);
-  for (uint32_t i = 0; i < half_rot; i++) freq[i] = powf(p->theta, -(2.0f * (float)i) / (float)p->rot_dim);
+  // (axes: 64-bit turns in its place)
+  std::vector<float> freq(std::max<uint32_t>(axes ? 2 * half_rot : half_rot, 1), 0.f);
+  std::vector<double> turns(axes ? half_rot : 0);
+  if (axes) {
+    axes_turns(axes, p, turns.data());
+    std::memcpy(freq.data(), turns.data(), half_rot * sizeof(double));
+  }
+  for (uint32_t i = 0; !axes && i < half_rot; i++) freq[i] = powf(p->theta, -(2.0f * (float)i) / (float)p->rot_dim);
   hipStream_t st = (hipStream_t)stream;
   if ((rc = kv->flush(st)) != LMH_OK) return rc;
   const int32_t *rs, *rp;
@@ -1425,6 +1474,14 @@ int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint6
   RopeGeom r{y.n_head, q_stride, p->flags, half_rot, p->eps, p->freq_scale, p->attn_factor,
              (p->flags & LMH_ROPE_Q_NORM) ? p->q_norm : nullptr, (p->flags & LMH_ROPE_K_NORM) ? p->k_norm : nullptr,
              apply ? p->freq_div : nullptr, (const float*)ex};
+  if (axes) {
+    r.positions = axes->positions;
+    r.turns = (const double*)ex;
+    r.n_rows = (uint32_t)n_rows;
+    r.n_axes = axes->n_axes;
+    r.interleaved = (axes->flags & LMH_ROPE_AXES_INTERLEAVED) ? 1u : 0u;
+    for (uint32_t a = 0; a < ROPE_MAX_AXES; a++) r.sec[a] = axes->sections[a];
+  }
   hipError_t e;
   LaunchEv ev;
   if ((e = kv->time_launch(LMH_KERNEL_ROPE_STORE, ev)) != hipSuccess) return kv->hip_fail(e, "event");
@@ -1432,6 +1489,20 @@ int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint6
                            d_lists + n_quads, (uint32_t)(lists.size() - n_quads), st, ev);
   if (e != hipSuccess) return kv->hip_fail(e, "kernel launch");
   return kv->release_rows(slot, st);
+}
+
+int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
+                          const float* k_in, const float* v_in, float* q_out, const lmh_rope_params* p,
+                          void* stream) {
+  return rope_impl(kv, layer, segs, n_segs, q_in, k_in, v_in, q_out, p, nullptr, stream);
+}
+
+int32_t lmh_qk_rope_store_axes(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
+                               const float* k_in, const float* v_in, float* q_out, const lmh_rope_params* p,
+                               const lmh_rope_axes* axes, void* stream) {
+  if (!kv) return LMH_INVALID_ARGUMENT;
+  if (!axes) return kv->fail(LMH_INVALID_ARGUMENT, "rope axes: null");
+  return rope_impl(kv, layer, segs, n_segs, q_in, k_in, v_in, q_out, p, axes, stream);
 }
 
 // What the planner needs to know of the kernel modules for a layer's geometry.
@@ -1447,13 +1518,41 @@ static void fill_kernel_facts(PlanIn& in, uint32_t kv_type, uint32_t hd, uint32_
   in.mfma_local_ok = decode_mfma_local_ok(kv_type, hd, hdv);
 }
 
-// lmh_attend and lmh_attend_noalloc. noalloc: split-K partials and the merge list go to the
+// A call with shaped scores: a unit launch whatever its segments, or the row layout's items.
+static void plan_scored(PlanIn& in, uint32_t kv_type, uint32_t layout) {
+  in.scored = true;
+  in.prefill_supported = false;
+  in.prefill_min_rows = in.decode_target_items = in.decode_min_tiles = 0;
+  for (uint32_t nb = 1; nb <= 2; nb++) in.unit_w[nb - 1] = scored_waves(kv_type, in.hd, in.hdv, layout, nb);
+}
+
+// The keys each row of a call with shaped scores sees, the window in them. n_rows: all; less: the first row whose
+// keys are not there.
+static uint64_t row_ranges(const lmh_seg* segs, uint64_t n_segs, uint64_t n_rows, uint64_t window, const uint32_t* row_lo,
+                           const uint32_t* row_hi, std::vector<KeyRange>& out) {
+  out.resize(n_rows);
+  for (uint64_t i = 0; i < n_segs; i++) {
+    const lmh_seg& sg = segs[i];
+    for (uint64_t j = 0; j < sg.n; j++) {
+      const uint64_t t = sg.start + j, pos = sg.pos0 + j;
+      const uint64_t behind = window > 0 && pos + 1 > window ? pos + 1 - window : 0;
+      const uint64_t lo = std::max<uint64_t>(behind, row_lo ? row_lo[t] : 0), hi = row_hi ? row_hi[t] : pos + 1;
+      if (hi > sg.pos0 + sg.n) return t;
+      out[t] = lo < hi ? KeyRange{(uint32_t)lo, (uint32_t)(hi - 1)} : KeyRange{1u, 0u};
+    }
+  }
+  return n_rows;
+}
+
+// lmh_attend, lmh_attend_noalloc and lmh_attend_scored (sp, whose scale and window are the call's). noalloc: split-K partials and the merge list go to the
 // device's no-allocation scratch (the split target capped to what it holds, a call that still
 // needs more is refused), the staged work list must fit the staging capacity reserved at
 // creation, and no timing events are made or recorded: the call allocates nothing.
 static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q,
-                           float* out, float scale, uint64_t window, void* stream, bool noalloc) {
+                           float* out, float scale, uint64_t window, void* stream, bool noalloc,
+                           const lmh_score_params* sp = nullptr) {
   if (!kv) return LMH_INVALID_ARGUMENT;
+  const char* const name = sp ? "lmh_attend_scored" : "lmh_attend";
   if (noalloc && !kv->scratch) return kv->fail(LMH_DEVICE_ERROR, "no-allocation scratch not resolved");
   // A captured graph would replay this call's kernels against a staging slot that later calls
   // overwrite (the work list is read from it when the kernels run), so capture is refused before
@@ -1461,8 +1560,8 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing((hipStream_t)stream, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone)
-      return kv->fail(LMH_UNSUPPORTED, "lmh_attend cannot be captured into a graph: its work list lives in a "
-                                       "staging slot that later calls reuse");
+      return kv->fail(LMH_UNSUPPORTED, std::string(name) + " cannot be captured into a graph: its work list lives in a "
+                                                            "staging slot that later calls reuse");
   }
   if (layer >= kv->layers.size()) return kv->fail(LMH_INVALID_ARGUMENT, "layer out of range");
   if (!std::isfinite(scale)) return kv->fail(LMH_INVALID_ARGUMENT, "scale must be finite");
@@ -1477,6 +1576,12 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
     return kv->fail(LMH_INVALID_ARGUMENT, "a window layer's attention window must be 1..its width");
   if ((rc = kv->check_window_rows(layer, segs, n_segs, window)) != LMH_OK) return rc;
   const uint32_t group = y.n_head / y.n_kv;
+  const bool ranged = sp && (sp->row_lo || sp->row_hi);
+  if (ranged) {
+    const uint64_t t = row_ranges(segs, n_segs, n_rows, window, sp->row_lo, sp->row_hi, kv->ranges);
+    if (t < n_rows)
+      return kv->fail(LMH_INVALID_ARGUMENT, "row " + std::to_string(t) + " sees keys past its segment's last position");
+  }
   hipStream_t st = (hipStream_t)stream;
   if (kv->decode_capacity[layer] == 0)
     kv->decode_capacity[layer] = decode_waves_per_cu(kv->kv_type, y.hd, y.hdv, group, y.layout) * kv->n_cu;
@@ -1511,9 +1616,18 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   pin.unit_waves_per_cu = [](const PlanIn& in, uint32_t nb) {
     return unit_waves_per_cu(in.device, in.kv_type, in.hd, in.hdv, in.layout, nb);
   };
+  if (sp) {
+    plan_scored(pin, kv->kv_type, y.layout);
+    pin.ranges = ranged ? kv->ranges.data() : nullptr;
+    pin.unit_waves_per_cu = [](const PlanIn& in, uint32_t nb) {
+      return scored_waves_per_cu(in.device, in.kv_type, in.hd, in.hdv, in.layout, nb);
+    };
+  }
   pin.device = kv->device;
   PlanOut& pl = kv->plan;
   plan_attend(pin, pl);
+  if (sp && !pl.items.empty() && y.layout != LAYOUT_ROWS)
+    return kv->fail(LMH_UNSUPPORTED, "lmh_attend_scored: more query heads or KV heads than a unit's record holds");
   const uint32_t ng = pl.ng, slots = pl.slots, pf_wg = pl.pf_wg, pf_per_wg = pl.pf_per_wg, max_pages = pl.max_pages;
   const size_t slot_bytes = (size_t)ng * (y.hdv + 4) * 4;
   if ((rc = kv->flush(st)) != LMH_OK) return rc;
@@ -1521,10 +1635,12 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   const size_t items_pad = (items_bytes + 255) / 256 * 256;
   const size_t merges_bytes = kv->plan.merges.size() * sizeof(MergeItem);
   const size_t merges_pad = (merges_bytes + 255) / 256 * 256;
-  // one staged payload: [decode items | merges | prefill items], or [merges | unit waves], the latter
-  // copied to the staging slot straight from the plan
+  // one staged payload: [decode items | merges | prefill items or ranges], or [merges | ranges | unit waves], the
+  // waves copied to the staging slot straight from the plan
   const size_t uwaves_bytes = kv->plan.uwaves.size() * sizeof(UnitWave);
-  kv->payload.resize(items_pad + merges_pad + kv->plan.pitems.size() * sizeof(PrefillItem));
+  const size_t ranges_bytes = ranged && uwaves_bytes ? (n_rows * sizeof(KeyRange) + 255) / 256 * 256 : 0;
+  kv->payload.resize(items_pad + merges_pad + kv->plan.pitems.size() * sizeof(PrefillItem) + ranges_bytes);
+  if (ranges_bytes) std::memcpy(kv->payload.data() + items_pad + merges_pad, kv->ranges.data(), n_rows * sizeof(KeyRange));
   if (items_bytes) std::memcpy(kv->payload.data(), kv->plan.items.data(), items_bytes);
   if (merges_bytes) std::memcpy(kv->payload.data() + items_pad, kv->plan.merges.data(), merges_bytes);
   if (!kv->plan.pitems.empty())
@@ -1564,6 +1680,15 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   r.group = group;
   r.ng = ng;
   r.scale_log2 = scale * 1.4426950408889634f;
+  ScoreGeom sg{};
+  if (sp) {
+    sg.slopes = sp->slopes;
+    sg.ranges = ranges_bytes ? (const uint2*)(ex + items_pad + merges_pad) : nullptr;
+    if (sp->cap > 0.f) {
+      sg.cap_log2 = sp->cap * 1.4426950408889634f;
+      r.scale_log2 = scale / sp->cap;
+    }
+  }
   r.window = (uint32_t)std::min<uint64_t>(window, 0xffffffffull);
   r.local_merge = pl.local;   // 0, or the waves per workgroup of a local-merge launch
   PrefillGeom pg{};
@@ -1603,15 +1728,17 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   }
   if (!overlap && !kv->plan.items.empty()) {
     if ((e = time_launch(LMH_KERNEL_DECODE, ev)) != hipSuccess) return kv->hip_fail(e, "event");
-    e = launch_decode(g, r, (const DecodeItem*)ex, (uint32_t)kv->plan.items.size(), q, out, part, mc, st,
-                      ev);
+    e = sp ? launch_scored_rows(g, r, sg, (const DecodeItem*)ex, (uint32_t)kv->plan.items.size(), q, out, part, mc, st, ev)
+           : launch_decode(g, r, (const DecodeItem*)ex, (uint32_t)kv->plan.items.size(), q, out, part, mc, st, ev);
     if (e != hipSuccess) return kv->hip_fail(e, "decode kernel");
   }
   if (uwaves_bytes) {
     const UnitGeom ug{y.n_head, group, r.scale_log2, r.window, ng, pl.u_shared ? 1u : 0u, part};
     if ((e = time_launch(LMH_KERNEL_PREFILL, ev)) != hipSuccess) return kv->hip_fail(e, "event");
-    e = launch_units(g, ug, pl.u_nb, pl.u_w, (const UnitWave*)(ex + items_pad + merges_pad), (uint32_t)(pl.uwaves.size() / pl.u_w),
-                     q, out, mc, st, ev);
+    const UnitWave* uw = (const UnitWave*)(ex + items_pad + merges_pad + ranges_bytes);
+    const uint32_t n_wg = (uint32_t)(pl.uwaves.size() / pl.u_w);
+    e = sp ? launch_scored_units(g, ug, sg, pl.u_nb, pl.u_w, uw, n_wg, q, out, mc, st, ev)
+           : launch_units(g, ug, pl.u_nb, pl.u_w, uw, n_wg, q, out, mc, st, ev);
     if (e != hipSuccess) return kv->hip_fail(e, "unit kernel");
   }
   if (!kv->plan.merges.empty()) {
@@ -1644,6 +1771,19 @@ int32_t lmh_attend(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_s
 int32_t lmh_attend_noalloc(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q,
                            float* out, float scale, uint64_t window, void* stream) {
   return attend_impl(kv, layer, segs, n_segs, q, out, scale, window, stream, true);
+}
+
+int32_t lmh_attend_scored(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q, float* out,
+                          const lmh_score_params* p, void* stream) {
+  if (!kv) return LMH_INVALID_ARGUMENT;
+  if (!p || p->abi_version != LMH_ABI_VERSION) return kv->fail(LMH_INVALID_ARGUMENT, "score params: null or ABI version");
+  if (p->reserved0) return kv->fail(LMH_INVALID_ARGUMENT, "score params: reserved0 must be 0");
+  if (!(p->cap >= 0.f) || !std::isfinite(p->cap)) return kv->fail(LMH_INVALID_ARGUMENT, "cap must be finite and not negative");
+  // (scale: tested with the call's other arguments)
+  if (p->cap > 0.f && std::isfinite(p->scale) && (!std::isfinite(p->scale / p->cap) || !std::isfinite(p->cap * 1.4426950408889634f)))
+    return kv->fail(LMH_INVALID_ARGUMENT, "scale / cap is out of range");
+  if ((uintptr_t)p->slopes % 4) return kv->fail(LMH_INVALID_ARGUMENT, "slopes must be 4-byte aligned");
+  return attend_impl(kv, layer, segs, n_segs, q, out, p->scale, p->window, stream, false, p);
 }
 
 // nullptr, or what is wrong with the options
@@ -1687,7 +1827,9 @@ int32_t lmh_kv_get_tuning(const lmh_kv* kv, lmh_attend_tuning* t) {
 
 // The planner alone on host data (no device): validates like lmh_kv_create / lmh_attend and plans as
 // lmh_attend would for a layer of this geometry.
-static int32_t plan_desc(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, PlanIn& in, PlanOut& o) {
+// scored: as lmh_attend_scored, with its row_lo / row_hi.
+static int32_t plan_desc(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, PlanIn& in, PlanOut& o, bool scored = false,
+                         const uint32_t* row_lo = nullptr, const uint32_t* row_hi = nullptr) {
   if (!d || d->abi_version != LMH_ABI_VERSION || (n_segs > 0 && !segs)) return LMH_INVALID_ARGUMENT;
   const uint32_t bt = d->block_tokens;
   if (d->kv_type > LMH_KV_BF16 || bt == 0 || (bt & (bt - 1)) != 0 || d->n_kv == 0 || d->n_head == 0 ||
@@ -1740,8 +1882,17 @@ static int32_t plan_desc(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n
   in.noalloc_stage = list_bytes(staging_bytes(in.bps), n_rows);
   in.list_units = true;
   fill_kernel_facts(in, d->kv_type, d->hd, d->hdv, d->n_head / d->n_kv, in.layout);
+  std::vector<KeyRange> ranges;
+  if (scored) {
+    plan_scored(in, in.kv_type, in.layout);
+    if (row_lo || row_hi) {
+      if (row_ranges(segs, n_segs, n_rows, d->window, row_lo, row_hi, ranges) < n_rows) return LMH_INVALID_ARGUMENT;
+      in.ranges = ranges.data();
+    }
+  }
   if (n_rows > 0) plan_attend(in, o);
   in.row_seq = in.row_pos = nullptr;   // the arrays end here
+  in.ranges = nullptr;
   return LMH_OK;
 }
 
@@ -1788,6 +1939,25 @@ int32_t lmh_plan_unit_waves(const lmh_plan_desc* d, const lmh_seg* segs, uint64_
   if (counts->n_waves > waves_cap || counts->n_merges > merges_cap) return LMH_INVALID_ARGUMENT;
   if (counts->n_waves) std::memcpy(waves, o.uwaves.data(), o.uwaves.size() * sizeof(UnitWave));
   if (counts->n_merges) std::memcpy(merges, o.merges.data(), o.merges.size() * sizeof(MergeItem));
+  return LMH_OK;
+}
+
+int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, const uint32_t* row_lo,
+                        const uint32_t* row_hi, uint32_t waves_per_cu, uint32_t* waves, uint64_t waves_cap, uint32_t* items,
+                        uint64_t items_cap, uint32_t* merges, uint64_t merges_cap, lmh_plan_wave_counts* counts,
+                        uint64_t* n_items) {
+  if (!counts || !n_items || waves_per_cu == 0) return LMH_INVALID_ARGUMENT;
+  PlanIn in;
+  PlanOut o;
+  in.unit_waves_given = waves_per_cu;
+  if (const int32_t rc = plan_desc(d, segs, n_segs, in, o, true, row_lo, row_hi); rc != LMH_OK) return rc;
+  *counts = lmh_plan_wave_counts{o.uwaves.size(), o.merges.size(), sizeof(UnitWave) / 4, sizeof(MergeItem) / 4,
+                                 o.u_w, o.u_nb, o.u_shared ? 1u : 0u, o.ng, o.slots, in.layout};
+  *n_items = o.items.size();
+  if (o.uwaves.size() > waves_cap || o.items.size() > items_cap || o.merges.size() > merges_cap) return LMH_INVALID_ARGUMENT;
+  if (!o.uwaves.empty()) std::memcpy(waves, o.uwaves.data(), o.uwaves.size() * sizeof(UnitWave));
+  if (!o.items.empty()) std::memcpy(items, o.items.data(), o.items.size() * sizeof(DecodeItem));
+  if (!o.merges.empty()) std::memcpy(merges, o.merges.data(), o.merges.size() * sizeof(MergeItem));
   return LMH_OK;
 }
 

@@ -222,6 +222,29 @@ __device__ inline float wave_sum(float x) {
   return x;
 }
 
+// cos and sin of pair i of a row whose axes have positions of their own, times attn_factor. The angle is
+// position * freq_scale * theta^(-2i/rot_dim) (/ freq_div) in 64 bits, as turns: in 32 the rounding of a far
+// position's angle alone moves it by 2^-24 of it (6e-3 at 100,000). Only its fraction goes on in 32 bits.
+__device__ inline float2 axes_factor(const RopeGeom& r, uint32_t row, uint32_t i) {
+  uint32_t a;
+  if (r.interleaved) {
+    const uint32_t m = i % r.n_axes;
+    uint32_t n = r.sec[0];
+#pragma unroll
+    for (uint32_t k = 1; k < ROPE_MAX_AXES; k++) n = m == k ? r.sec[k] : n;
+    a = m != 0 && i < r.n_axes * n ? m : 0;
+  } else {
+    const uint32_t e0 = r.sec[0], e1 = e0 + r.sec[1], e2 = e1 + r.sec[2];
+    a = (i >= e0) + (i >= e1) + (i >= e2);
+  }
+  double t = r.turns[i] * (double)r.positions[(size_t)a * r.n_rows + row];
+  if (r.freq_div) t /= (double)r.freq_div[i];
+  t -= rint(t);
+  float sn, cn;
+  sincospif((float)(2.0 * t), &sn, &cn);
+  return make_float2(cn * r.attn_factor, sn * r.attn_factor);
+}
+
 // One workgroup (4 waves) per row. The row's heads (Q, then K, then V; hd == hdv) are pulled into
 // LDS in chunks of up to ROPE_LDS_FLOATS floats with 16-byte loads spread over all threads, so one
 // round trip fetches a whole row. Meanwhile the rotation factors are computed once per row: the
@@ -266,6 +289,10 @@ __global__ __launch_bounds__(256) void qk_rope_store_kernel(PageGeom g, RopeGeom
     if (i0 == 0) {
       sl = locate(g, row_seq[row], pos);
       for (uint32_t i = tid; i < r.half_rot; i += blockDim.x) {
+        if (r.positions) {
+          cs[i] = axes_factor(r, row, i);
+          continue;
+        }
         float angle = (float)pos * r.freq_scale * r.freq[i];
         if (r.freq_div) angle = angle / r.freq_div[i];
         double sn, cn;
@@ -349,6 +376,10 @@ __global__ __launch_bounds__(256) void qk_rope_store_reg_kernel(PageGeom g, Rope
     xs[j] = it < n_items ? *(const fv*)(src_of(it) + lane * VPL) : fv{};
   }
   for (uint32_t i = tid; i < r.half_rot; i += blockDim.x) {
+    if (r.positions) {
+      cs[i] = axes_factor(r, row, i);
+      continue;
+    }
     float angle = (float)pos * r.freq_scale * r.freq[i];
     if (r.freq_div) angle = angle / r.freq_div[i];
     float sn, cn;
@@ -603,6 +634,10 @@ __device__ void rope_tokens(const PageGeom& g, const RopeGeom& r, float2 (*cs)[R
   const uint32_t half = r.half_rot;
   for (uint32_t i = tid; i < NT * half; i += blockDim.x) {
     const uint32_t t = i / half, ii = i - t * half;
+    if (r.positions) {
+      cs[t][ii] = axes_factor(r, row0 + t, ii);
+      continue;
+    }
     float angle = (float)(pos0 + t) * r.freq_scale * r.freq[ii];
     if (r.freq_div) angle = angle / r.freq_div[ii];
     float sn, cn;
@@ -841,6 +876,10 @@ __device__ void rope_quad_slots(const PageGeom& g, const RopeGeom& r, float2 (*c
   const uint32_t half = r.half_rot;
   for (uint32_t i = tid; i < 4 * half; i += blockDim.x) {
     const uint32_t tk = i / half, ii = i - tk * half;
+    if (r.positions) {
+      cs[tk][ii] = axes_factor(r, row0 + tk, ii);
+      continue;
+    }
     float angle = (float)(pos0 + tk) * r.freq_scale * r.freq[ii];
     if (r.freq_div) angle = angle / r.freq_div[ii];
     float sn, cn;

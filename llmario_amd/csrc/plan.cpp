@@ -92,7 +92,8 @@ void for_each_merge(const PrefillItem& it, uint64_t group, uint32_t k, F&& f, ui
 // decode items.
 bool plan_units(const PlanIn& in, PlanOut& o) {
   // explicit split settings address the prefill and decode kernels
-  if (!in.unit_w[0] || in.bt_shift < 4 || in.prefill_min_rows || in.decode_target_items || in.decode_min_tiles) return false;
+  if (!in.unit_w[0] || in.bt_shift < 4) return false;
+  if (!in.scored && (in.prefill_min_rows || in.decode_target_items || in.decode_min_tiles)) return false;
   const uint64_t group = in.n_head / in.n_kv;
   if (group > 0xffff || in.n_kv > 0xffff) return false;   // a wave's record packs both
   const bool f32 = in.kv_type == LMH_KV_F32, pf_ok = in.scale > 0.f && in.layout == LAYOUT_TILES && in.prefill_supported;
@@ -112,20 +113,43 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
   }
   // Decode rows alone: the row layout's, and f32 pages' of wide groups (16 rows x 3,000 keys, hd 128:
   // group 8 166.6 -> 103.0 us; group 4 113.0 -> 102.5 but 16 x 700 36.2 -> 37.2, group 1 77.9 -> 101.4).
-  if (!multi && in.layout == LAYOUT_TILES && !(f32 && group >= 8 && max_pages > 16)) return false;
+  if (!in.scored && !multi && in.layout == LAYOUT_TILES && !(f32 && group >= 8 && max_pages > 16)) return false;
   // Short segments on the decode item's pages: when sharing the walks saves the device's waves ten
   // tiles each or more (32/8 heads, hd 128, f16: 8 x 2 rows of 2,000 keys 20.4 -> 24.6 us, saves 8;
   // 5 rows of 6,000 24.4 -> 20.3, saves 11; 32 x 3 of 700 43.2 -> 23.6, saves 22).
-  if (in.layout == LAYOUT_TILES && !f32 && (steps_rows - std::min(steps_rows, in.unit_w[1] ? steps32 : steps16)) * in.n_kv < 40ull * in.n_cu)
+  if (!in.scored && in.layout == LAYOUT_TILES && !f32 && (steps_rows - std::min(steps_rows, in.unit_w[1] ? steps32 : steps16)) * in.n_kv < 40ull * in.n_cu)
     return false;
   // (o is written once the call is taken: one given back keeps what the other planners set)
-  const uint32_t nb = in.unit_w[1] && 4 * steps32 < 3 * steps16 ? 2 : 1;
-  const uint32_t KT = f32 ? 1 : 2, cols = 16 * nb;
   // A segment's column blocks; a unit is a block for one KV head.
   struct Block {
     PrefillItem it;
     uint32_t ns;   // steps
   };
+  const uint32_t KT = f32 ? 1 : 2;
+  // the pages that the rows t0 .. t1 of a segment see, first and last (rows that see nothing: one page, masked)
+  auto pages_seen = [&](const lmh_seg& sg, uint64_t t0, uint64_t t1) -> std::pair<uint64_t, uint64_t> {
+    if (!in.ranges) return {key_lo(sg.pos0 + t0, in.window) / 16, (sg.pos0 + t1) / 16};
+    uint64_t first = ~0ull, last = 0;
+    for (uint64_t t = t0; t <= t1; t++) {
+      const KeyRange& r = in.ranges[sg.start + t];
+      if (r.first > r.last) continue;
+      first = std::min<uint64_t>(first, r.first);
+      last = std::max<uint64_t>(last, r.last);
+    }
+    if (first > last) first = last = sg.pos0 + t0;
+    return {first / 16, last / 16};
+  };
+  if (in.ranges) {   // the walks by the rows' own ranges
+    steps16 = steps32 = 0;
+    for (uint32_t w = 1; w <= 2; w++)
+      for (uint64_t i = 0; i < in.n_segs; i++)
+        for (uint64_t n_cols = in.segs[i].n * group, c0 = 0; c0 < n_cols; c0 += 16 * w) {
+          const auto p = pages_seen(in.segs[i], c0 / group, (std::min<uint64_t>(c0 + 16 * w, n_cols) - 1) / group);
+          (w == 1 ? steps16 : steps32) += p.second - p.first + 1;
+        }
+  }
+  const uint32_t nb = in.unit_w[1] && 4 * steps32 < 3 * steps16 ? 2 : 1;
+  const uint32_t cols = 16 * nb;
   std::vector<Block> blocks;
   std::vector<uint32_t> seg0;   // each segment's first block
   uint64_t total = 0, max_ns = 0;
@@ -137,14 +161,15 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
       Block b{};
       b.it.n_col = (uint32_t)std::min<uint64_t>(cols, n_cols - c0);
       const uint64_t t0 = c0 / group, t1 = (c0 + b.it.n_col - 1) / group;
-      const uint64_t page_lo = key_lo(sg.pos0 + t0, in.window) / 16;
+      const auto pages = pages_seen(sg, t0, t1);
+      const uint64_t page_lo = pages.first;
       b.it.seq = (uint32_t)sg.seq;
       b.it.row0 = (uint32_t)(sg.start + t0);
       b.it.pos0 = (uint32_t)(sg.pos0 + t0);
       b.it.n_tok = (uint32_t)(t1 - t0 + 1);
       b.it.c_off = (uint32_t)(c0 % group);
       b.it.page0 = (uint32_t)page_lo;
-      b.it.n_pages = (uint32_t)((sg.pos0 + t1) / 16 - page_lo + 1);
+      b.it.n_pages = (uint32_t)(pages.second - page_lo + 1);
       b.it.slot = NO_SLOT;
       b.ns = (b.it.n_pages + KT - 1) / KT;
       total += b.ns;
@@ -370,7 +395,7 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
     const uint32_t ns = (pages_of(m) + KT - 1) / KT, n = std::min(m.n, ns);
     walk = std::max<uint64_t>(walk, (uint64_t)(ns + n - 1) / n * KT);
   }
-  if (!rounds && 2 * walk > 3 * item_walk * (mfma_items ? 1 : in.layout == LAYOUT_ROWS ? 20 : 4) + 16) return false;
+  if (!in.scored && !rounds && 2 * walk > 3 * item_walk * (mfma_items ? 1 : in.layout == LAYOUT_ROWS ? 20 : 4) + 16) return false;
   o.ng = (uint32_t)group;   // a piece's partial slot holds the group's heads
   o.u_nb = nb;
   o.u_w = W;
@@ -716,9 +741,16 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
 
   // ---- decode work list: per (row, KV head, head block), the key range [lo, pos] cut into
   // chunks of whole 16-token tiles, spread evenly; rows whose range fits one chunk write the output.
-  auto row_tiles = [&](uint64_t t) {
+  // a row's first key and the one after its last, and its tiles (a row that sees none: one, of no keys)
+  auto row_keys = [&](uint64_t t) -> std::pair<uint64_t, uint64_t> {
     const uint64_t pos = (uint64_t)in.row_pos[t];
-    return pos / 16 - key_lo(pos, window) / 16 + 1;
+    if (!in.ranges) return {key_lo(pos, window), pos + 1};
+    const KeyRange& r = in.ranges[t];
+    return r.first > r.last ? std::make_pair(pos, pos) : std::make_pair<uint64_t, uint64_t>(r.first, r.last + 1ull);
+  };
+  auto row_tiles = [&](uint64_t t) -> uint64_t {
+    const auto k = row_keys(t);
+    return k.first == k.second ? 1 : (k.second - 1) / 16 - k.first / 16 + 1;
   };
   uint64_t total_tiles = 0;
   for (uint64_t t = 0; t < n_rows; t++)
@@ -815,9 +847,9 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
   };
   std::vector<Piece> pieces;
   auto cut_row = [&](uint64_t t, uint64_t k) {
-    const uint64_t pos = (uint64_t)in.row_pos[t];
-    const uint64_t lo = key_lo(pos, window), hi = pos + 1;
-    const uint64_t tlo = lo / 16, n_t = pos / 16 - tlo + 1;
+    const auto keys = row_keys(t);
+    const uint64_t lo = keys.first, hi = keys.second;
+    const uint64_t tlo = lo / 16, n_t = row_tiles(t);
     const uint64_t seq = (uint64_t)in.row_seq[t];
     const uint64_t q = n_t / k, r = n_t % k;
     pieces.clear();

@@ -13,6 +13,11 @@
 
 namespace lmh {
 
+// The keys a row sees: first .. last (first > last: none).
+struct KeyRange {
+  uint32_t first, last;
+};
+
 struct PlanIn {
   // the call's stacked rows (sequence and position of each) and its segments
   const int32_t* row_seq = nullptr;
@@ -29,6 +34,8 @@ struct PlanIn {
   uint32_t layout = LAYOUT_TILES;   // LAYOUT_TILES / LAYOUT_ROWS
   uint32_t kv_type = 0;             // LMH_KV_*
   uint64_t window = 0;              // the call's attention window (0: none)
+  const KeyRange* ranges = nullptr; // shaped scores: the keys each row sees, the window in it (null: those of the window)
+  bool scored = false;              // lmh_attend_scored: a unit launch of any call, or the row layout's items
   float scale = 0.f;
   // the device
   uint32_t n_cu = 1;

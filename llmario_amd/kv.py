@@ -66,6 +66,53 @@ def _segs(segs):
     return arr, len(segs)
 
 
+def _ptr(t):
+    return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+class RowRanges:
+    """The keys each row of a batch sees, lo <= key < hi, packed once for the C ABI (reuse it across layers).
+
+    lo, hi: one integer per stacked row (sequences or CPU integer tensors), or None (0 / the row's position + 1)."""
+
+    def __init__(self, lo=None, hi=None):
+        self.lo, self.hi = self._pack(lo), self._pack(hi)
+        if self.lo is not None and self.hi is not None and len(self.lo) != len(self.hi):
+            raise ValueError("lo and hi must have one value per row each")
+        self.n = len(self.lo if self.lo is not None else self.hi) if (self.lo is not None or self.hi is not None) else None
+
+    @staticmethod
+    def _pack(x):
+        if x is None:
+            return None
+        x = [int(i) for i in (x.tolist() if hasattr(x, "tolist") else x)]
+        if any(i < 0 or i > 0xffffffff for i in x):
+            raise ValueError("a row's keys are given by unsigned 32-bit positions")
+        return (N.u32 * max(len(x), 1))(*x) if x else (N.u32 * 0)()
+
+    @classmethod
+    def of(cls, segs, prefix=None, documents=None):
+        """The ranges of a batch's rows, causal but for what is given per segment: ``prefix`` (None or the end of a
+        span from position 0 whose tokens see each other) and ``documents`` (None or the positions at which packed
+        documents begin: a row sees its own document only)."""
+        segs = segs.segs if isinstance(segs, Segments) else [tuple(map(int, s)) for s in segs]
+        lo, hi = [], []
+        for i, (_, _, n, pos0) in enumerate(segs):
+            end = int(prefix[i] or 0) if prefix is not None else 0
+            if end > pos0 + n:
+                raise ValueError("a prefix may not end past its segment")
+            starts = sorted(int(d) for d in (documents[i] or ())) if documents is not None else []
+            at = 0
+            for pos in range(pos0, pos0 + n):
+                while at < len(starts) and starts[at] <= pos:
+                    at += 1
+                first = starts[at - 1] if at else 0
+                last = max(pos + 1, end) if pos < end else pos + 1
+                lo.append(first)
+                hi.append(min(last, starts[at]) if at < len(starts) else last)
+        return cls(lo, hi)
+
+
 class HipKvCache:
     """The device page pool of one model's attention layers (KvCache on the GPU)."""
 
@@ -254,15 +301,43 @@ class HipKvCache:
         Q written to q_out [n_rows, n_head, hd], K and V stored into the cache. q_in is
         [n_rows, n_head, q_stride or hd], k_in [n_rows, n_kv, hd], v_in [n_rows, n_kv, hdv] f32 cuda
         tensors; q_norm / k_norm are [hd] weights (None = no norm), freq_div [rot_dim/2] or None."""
+        p = self._rope_params(layer, rot_dim, theta, neox, rope, q_norm, k_norm, v_norm, eps, freq_scale, attn_factor,
+                              q_stride, freq_div)
+        arr, n = _segs(segs)
+        self._check(N.lib().lmh_qk_rope_store(self.h, layer, arr, n, _ptr(q_in), _ptr(k_in), _ptr(v_in),
+                                              _ptr(q_out), C.byref(p), _stream_ptr(stream)))
+
+    def qk_rope_store_axes(self, layer: int, segs, q_in, k_in, v_in, q_out, positions, sections, *,
+                           interleaved: bool = False, own_freq: bool = False, rot_dim: int = 0, theta: float = 10000.0,
+                           neox: bool = False, q_norm=None, k_norm=None, v_norm: bool = False, eps: float = 1e-6,
+                           freq_scale: float = 1.0, attn_factor: float = 1.0, q_stride: int = 0, freq_div=None,
+                           stream=None):
+        """qk_rope_store rotated at positions of several axes: positions is an int32 cuda tensor [n_axes, n_rows],
+        sections the pairs of each axis (one axis after the other, or with `interleaved` by turns; `own_freq`: each
+        axis has frequencies of its own). The rows are stored at their sequence positions, as the segments give them."""
+        import torch
+        arr, n = _segs(segs)
+        sections = [int(x) for x in sections]
+        if not 1 <= len(sections) <= 4 or min(sections) < 0:
+            raise ValueError("sections: the pairs of 1 to 4 axes")
+        n_rows = sum(int(s.n) for s in arr[:n])
+        if positions.dtype != torch.int32 or not positions.is_cuda or not positions.is_contiguous() or \
+                tuple(positions.shape) != (len(sections), n_rows):
+            raise ValueError("positions must be a contiguous int32 cuda tensor [n_axes, n_rows]")
+        p = self._rope_params(layer, rot_dim, theta, neox, True, q_norm, k_norm, v_norm, eps, freq_scale, attn_factor,
+                              q_stride, freq_div)
+        flags = (N.ROPE_AXES_INTERLEAVED if interleaved else 0) | (N.ROPE_AXES_OWN_FREQ if own_freq else 0)
+        x = N.RopeAxes(N.ABI_VERSION, len(sections), flags, (N.u32 * 4)(*sections), 0, positions.data_ptr())
+        self._check(N.lib().lmh_qk_rope_store_axes(self.h, layer, arr, n, _ptr(q_in), _ptr(k_in), _ptr(v_in),
+                                                   _ptr(q_out), C.byref(p), C.byref(x), _stream_ptr(stream)))
+
+    def _rope_params(self, layer, rot_dim, theta, neox, rope, q_norm, k_norm, v_norm, eps, freq_scale, attn_factor,
+                     q_stride, freq_div):
         hd = self.layers[layer].hd if 0 <= layer < len(self.layers) else 0  # the library checks the layer
         flags = (N.ROPE_APPLY if rope else 0) | (N.ROPE_NEOX if neox else 0) | (N.ROPE_V_NORM if v_norm else 0)
         flags |= (N.ROPE_Q_NORM if q_norm is not None else 0) | (N.ROPE_K_NORM if k_norm is not None else 0)
-        ptr = lambda t: C.c_void_p(t.data_ptr()) if t is not None else None
-        p = N.RopeParams(N.ABI_VERSION, flags, int(rot_dim or hd), int(q_stride), float(eps), float(theta),
-                         float(freq_scale), float(attn_factor), ptr(q_norm), ptr(k_norm), ptr(freq_div))
-        arr, n = _segs(segs)
-        self._check(N.lib().lmh_qk_rope_store(self.h, layer, arr, n, ptr(q_in), ptr(k_in), ptr(v_in),
-                                              ptr(q_out), C.byref(p), _stream_ptr(stream)))
+        return N.RopeParams(N.ABI_VERSION, flags, int(rot_dim or hd), int(q_stride), float(eps), float(theta),
+                            float(freq_scale), float(attn_factor), _ptr(q_norm), _ptr(k_norm), _ptr(freq_div))
 
     def attend(self, layer: int, segs, q, out, scale: float, window: int = 0, stream=None):
         """q: [n_rows, n_head, hd] f32 cuda tensor; out: [n_rows, n_head, hdv] f32."""
@@ -278,6 +353,24 @@ class HipKvCache:
         self._check(N.lib().lmh_attend_noalloc(self.h, layer, arr, n, C.c_void_p(q.data_ptr()),
                                                C.c_void_p(out.data_ptr()), float(scale), int(window or 0),
                                                _stream_ptr(stream)))
+
+    def attend_scored(self, layer: int, segs, q, out, scale: float, *, window: int = 0, cap: float = 0.0, slopes=None,
+                      ranges=None, stream=None):
+        """lmh_attend_scored: attend whose scores are capped, cap * tanh(s / cap) (cap 0: not), lose
+        slopes[head] * |position - key| (slopes: [n_head] f32 cuda tensor or None), and whose rows see the keys that
+        `ranges` (RowRanges, or None: causal) and `window` leave them; a row that sees none is zeros."""
+        arr, n = _segs(segs)
+        if ranges is not None and ranges.n is not None and ranges.n != sum(int(s.n) for s in arr[:n]):
+            raise ValueError(f"ranges of {ranges.n} rows for a batch of {sum(int(s.n) for s in arr[:n])}")
+        if slopes is not None and 0 <= layer < len(self.layers):   # the library checks the layer
+            import torch
+            if slopes.dtype != torch.float32 or not slopes.is_cuda or not slopes.is_contiguous() or slopes.numel() != self.layers[layer].n_head:
+                raise ValueError("slopes must be a contiguous f32 cuda tensor of n_head values")
+        p = N.ScoreParams(N.ABI_VERSION, 0, float(scale), float(cap or 0.0), slopes.data_ptr() if slopes is not None else None,
+                          C.cast(ranges.lo, N.P) if ranges is not None and ranges.lo is not None else None,
+                          C.cast(ranges.hi, N.P) if ranges is not None and ranges.hi is not None else None, int(window or 0))
+        self._check(N.lib().lmh_attend_scored(self.h, layer, arr, n, C.c_void_p(q.data_ptr()), C.c_void_p(out.data_ptr()),
+                                              C.byref(p), _stream_ptr(stream)))
 
     def set_tuning(self, *, prefill_p_f16: bool | None = None, prefill_min_rows: int | None = None,
                    decode_target_items: int | None = None, decode_min_tiles: int | None = None,
