@@ -180,8 +180,8 @@ SIGNATURES = {
     "lmh_kv_set_tuning": (i32, [P, C.POINTER(AttendTuning)]),
     "lmh_kv_get_tuning": (i32, [P, C.POINTER(AttendTuning)]),
     "lmh_plan_unit_waves": (i32, [C.POINTER(PlanDesc), P, u64, u32, P, u64, P, u64, C.POINTER(PlanWaveCounts)]),
-    "lmh_plan_scored": (i32, [C.POINTER(PlanDesc), P, u64, P, P, u32, P, u64, P, u64, P, u64, C.POINTER(PlanWaveCounts),
-                              C.POINTER(u64)]),
+    "lmh_plan_scored": (i32, [C.POINTER(PlanDesc), P, u64, P, P, u32, P, u64, P, u64, P, u64, P, u64, C.POINTER(PlanWaveCounts),
+                              C.POINTER(u64), C.POINTER(u64)]),
     "lmh_plan_attend": (i32, [C.POINTER(PlanDesc), P, u64, P, u64, P, u64, P, u64, C.POINTER(PlanCounts)]),
     "lmh_kv_set_timing": (i32, [P, i32]),
     "lmh_kv_kernel_time": (i32, [P, u32, C.POINTER(C.c_double), C.POINTER(u64)]),

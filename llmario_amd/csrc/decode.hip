@@ -27,6 +27,7 @@
 //
 // f32 pages (VALU): lane per key for Q.K, lane per dim for P.V, fp32 throughout.
 #include "decode_tile.h"
+#include "score.h"
 
 #include <mutex>
 #include <unordered_map>
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_rows_kernel(PageGeom g, Row
   const uint32_t pos = SC ? (uint32_t)r.row_pos[it.row] : 0u;
 #pragma unroll
   for (int h = 0; h < RNG; h++) {
-    slope[h] = SC && sc.slopes && h < (int)nh ? sc.slopes[it.kvh * r.group + it.h0 + h] * 1.4426950408889634f : 0.f;
+    slope[h] = SC && sc.slopes && h < (int)nh ? sc.slopes[it.kvh * r.group + it.h0 + h] * LOG2E : 0.f;
     m[h] = -INFINITY;
     l[h] = 0.f;
 #pragma unroll
@@ -580,8 +581,10 @@ __global__ __launch_bounds__(64 * WAVES) void decode_rows_kernel(PageGeom g, Row
       if (h >= (int)nh) break;
       float sv = s[h] * r.scale_log2;
       if constexpr (SC) {
-        if (sc.cap_log2 > 0.f) sv = sc.cap_log2 * tanhf(sv);
-        if (sc.slopes) sv = fmaf(-slope[h], fabsf((float)(int)(kk - pos)), sv);
+        float u[1] = {sv};
+        if (sc.cap_log2 > 0.f) cap_scores<1>(u, sc.cap_log2);
+        if (sc.slopes) bias_scores<1>(u, slope[h], (float)(int)(kk - pos), [](int) { return 0.f; });
+        sv = u[0];
       }
       sv = valid ? sv : -INFINITY;
       float cm = sv;

@@ -1524,6 +1524,7 @@ static void plan_scored(PlanIn& in, uint32_t kv_type, uint32_t layout) {
   in.prefill_supported = false;
   in.prefill_min_rows = in.decode_target_items = in.decode_min_tiles = 0;
   for (uint32_t nb = 1; nb <= 2; nb++) in.unit_w[nb - 1] = scored_waves(kv_type, in.hd, in.hdv, layout, nb);
+  in.prompt_cols = in.bt_shift >= 4 ? scored_prompt_cols(kv_type, in.hd, in.hdv, layout) : 0;
 }
 
 // The keys each row of a call with shaped scores sees, the window in them. n_rows: all; less: the first row whose
@@ -1626,7 +1627,7 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   pin.device = kv->device;
   PlanOut& pl = kv->plan;
   plan_attend(pin, pl);
-  if (sp && !pl.items.empty() && y.layout != LAYOUT_ROWS)
+  if (sp && y.layout != LAYOUT_ROWS && (!pl.items.empty() || (pl.uwaves.empty() && pl.prompts.empty())))
     return kv->fail(LMH_UNSUPPORTED, "lmh_attend_scored: more query heads or KV heads than a unit's record holds");
   const uint32_t ng = pl.ng, slots = pl.slots, pf_wg = pl.pf_wg, pf_per_wg = pl.pf_per_wg, max_pages = pl.max_pages;
   const size_t slot_bytes = (size_t)ng * (y.hdv + 4) * 4;
@@ -1635,12 +1636,15 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   const size_t items_pad = (items_bytes + 255) / 256 * 256;
   const size_t merges_bytes = kv->plan.merges.size() * sizeof(MergeItem);
   const size_t merges_pad = (merges_bytes + 255) / 256 * 256;
-  // one staged payload: [decode items | merges | prefill items or ranges], or [merges | ranges | unit waves], the
+  // one staged payload: [decode items | merges | prefill items], or [merges | ranges | prompts | unit waves], the
   // waves copied to the staging slot straight from the plan
   const size_t uwaves_bytes = kv->plan.uwaves.size() * sizeof(UnitWave);
-  const size_t ranges_bytes = ranged && uwaves_bytes ? (n_rows * sizeof(KeyRange) + 255) / 256 * 256 : 0;
-  kv->payload.resize(items_pad + merges_pad + kv->plan.pitems.size() * sizeof(PrefillItem) + ranges_bytes);
+  const size_t prompts_bytes = (kv->plan.prompts.size() * sizeof(PrefillItem) + 255) / 256 * 256;
+  const size_t ranges_bytes = ranged && uwaves_bytes + prompts_bytes ? (n_rows * sizeof(KeyRange) + 255) / 256 * 256 : 0;
+  kv->payload.resize(items_pad + merges_pad + kv->plan.pitems.size() * sizeof(PrefillItem) + ranges_bytes + prompts_bytes);
   if (ranges_bytes) std::memcpy(kv->payload.data() + items_pad + merges_pad, kv->ranges.data(), n_rows * sizeof(KeyRange));
+  if (prompts_bytes)
+    std::memcpy(kv->payload.data() + items_pad + merges_pad + ranges_bytes, kv->plan.prompts.data(), kv->plan.prompts.size() * sizeof(PrefillItem));
   if (items_bytes) std::memcpy(kv->payload.data(), kv->plan.items.data(), items_bytes);
   if (merges_bytes) std::memcpy(kv->payload.data() + items_pad, kv->plan.merges.data(), merges_bytes);
   if (!kv->plan.pitems.empty())
@@ -1732,10 +1736,16 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
            : launch_decode(g, r, (const DecodeItem*)ex, (uint32_t)kv->plan.items.size(), q, out, part, mc, st, ev);
     if (e != hipSuccess) return kv->hip_fail(e, "decode kernel");
   }
-  if (uwaves_bytes) {
-    const UnitGeom ug{y.n_head, group, r.scale_log2, r.window, ng, pl.u_shared ? 1u : 0u, part};
+  const UnitGeom ug{y.n_head, group, r.scale_log2, r.window, ng, pl.u_shared ? 1u : 0u, part};
+  if (prompts_bytes) {
     if ((e = time_launch(LMH_KERNEL_PREFILL, ev)) != hipSuccess) return kv->hip_fail(e, "event");
-    const UnitWave* uw = (const UnitWave*)(ex + items_pad + merges_pad + ranges_bytes);
+    e = launch_scored_prompts(g, ug, sg, (const PrefillItem*)(ex + items_pad + merges_pad + ranges_bytes), (uint32_t)pl.prompts.size(),
+                              q, out, uwaves_bytes ? MergeCopy{} : mc, st, ev);
+    if (e != hipSuccess) return kv->hip_fail(e, "prompt kernel");
+  }
+  if (uwaves_bytes) {
+    if ((e = time_launch(LMH_KERNEL_PREFILL, ev)) != hipSuccess) return kv->hip_fail(e, "event");
+    const UnitWave* uw = (const UnitWave*)(ex + items_pad + merges_pad + ranges_bytes + prompts_bytes);
     const uint32_t n_wg = (uint32_t)(pl.uwaves.size() / pl.u_w);
     e = sp ? launch_scored_units(g, ug, sg, pl.u_nb, pl.u_w, uw, n_wg, q, out, mc, st, ev)
            : launch_units(g, ug, pl.u_nb, pl.u_w, uw, n_wg, q, out, mc, st, ev);
@@ -1944,9 +1954,9 @@ int32_t lmh_plan_unit_waves(const lmh_plan_desc* d, const lmh_seg* segs, uint64_
 
 int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, const uint32_t* row_lo,
                         const uint32_t* row_hi, uint32_t waves_per_cu, uint32_t* waves, uint64_t waves_cap, uint32_t* items,
-                        uint64_t items_cap, uint32_t* merges, uint64_t merges_cap, lmh_plan_wave_counts* counts,
-                        uint64_t* n_items) {
-  if (!counts || !n_items || waves_per_cu == 0) return LMH_INVALID_ARGUMENT;
+                        uint64_t items_cap, uint32_t* prompts, uint64_t prompts_cap, uint32_t* merges, uint64_t merges_cap,
+                        lmh_plan_wave_counts* counts, uint64_t* n_items, uint64_t* n_prompts) {
+  if (!counts || !n_items || !n_prompts || waves_per_cu == 0) return LMH_INVALID_ARGUMENT;
   PlanIn in;
   PlanOut o;
   in.unit_waves_given = waves_per_cu;
@@ -1954,9 +1964,11 @@ int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_
   *counts = lmh_plan_wave_counts{o.uwaves.size(), o.merges.size(), sizeof(UnitWave) / 4, sizeof(MergeItem) / 4,
                                  o.u_w, o.u_nb, o.u_shared ? 1u : 0u, o.ng, o.slots, in.layout};
   *n_items = o.items.size();
-  if (o.uwaves.size() > waves_cap || o.items.size() > items_cap || o.merges.size() > merges_cap) return LMH_INVALID_ARGUMENT;
+  *n_prompts = o.prompts.size();
+  if (o.uwaves.size() > waves_cap || o.items.size() > items_cap || o.prompts.size() > prompts_cap || o.merges.size() > merges_cap) return LMH_INVALID_ARGUMENT;
   if (!o.uwaves.empty()) std::memcpy(waves, o.uwaves.data(), o.uwaves.size() * sizeof(UnitWave));
   if (!o.items.empty()) std::memcpy(items, o.items.data(), o.items.size() * sizeof(DecodeItem));
+  if (!o.prompts.empty()) std::memcpy(prompts, o.prompts.data(), o.prompts.size() * sizeof(PrefillItem));
   if (!o.merges.empty()) std::memcpy(merges, o.merges.data(), o.merges.size() * sizeof(MergeItem));
   return LMH_OK;
 }

@@ -88,6 +88,20 @@ void for_each_merge(const PrefillItem& it, uint64_t group, uint32_t k, F&& f, ui
   }
 }
 
+// The pages that rows t0 .. t1 of a segment see, first and last (rows that see nothing: the page of the first).
+std::pair<uint64_t, uint64_t> pages_seen(const PlanIn& in, const lmh_seg& sg, uint64_t t0, uint64_t t1) {
+  if (!in.ranges) return {key_lo(sg.pos0 + t0, in.window) / 16, (sg.pos0 + t1) / 16};
+  uint64_t first = ~0ull, last = 0;
+  for (uint64_t t = t0; t <= t1; t++) {
+    const KeyRange& r = in.ranges[sg.start + t];
+    if (r.first > r.last) continue;
+    first = std::min<uint64_t>(first, r.first);
+    last = std::max<uint64_t>(last, r.last);
+  }
+  if (first > last) first = last = sg.pos0 + t0;
+  return {first / 16, last / 16};
+}
+
 // The call as one unit launch (units.hip), when that is the faster way; false: as prefill units and
 // decode items.
 bool plan_units(const PlanIn& in, PlanOut& o) {
@@ -126,25 +140,12 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
     uint32_t ns;   // steps
   };
   const uint32_t KT = f32 ? 1 : 2;
-  // the pages that the rows t0 .. t1 of a segment see, first and last (rows that see nothing: one page, masked)
-  auto pages_seen = [&](const lmh_seg& sg, uint64_t t0, uint64_t t1) -> std::pair<uint64_t, uint64_t> {
-    if (!in.ranges) return {key_lo(sg.pos0 + t0, in.window) / 16, (sg.pos0 + t1) / 16};
-    uint64_t first = ~0ull, last = 0;
-    for (uint64_t t = t0; t <= t1; t++) {
-      const KeyRange& r = in.ranges[sg.start + t];
-      if (r.first > r.last) continue;
-      first = std::min<uint64_t>(first, r.first);
-      last = std::max<uint64_t>(last, r.last);
-    }
-    if (first > last) first = last = sg.pos0 + t0;
-    return {first / 16, last / 16};
-  };
   if (in.ranges) {   // the walks by the rows' own ranges
     steps16 = steps32 = 0;
     for (uint32_t w = 1; w <= 2; w++)
       for (uint64_t i = 0; i < in.n_segs; i++)
         for (uint64_t n_cols = in.segs[i].n * group, c0 = 0; c0 < n_cols; c0 += 16 * w) {
-          const auto p = pages_seen(in.segs[i], c0 / group, (std::min<uint64_t>(c0 + 16 * w, n_cols) - 1) / group);
+          const auto p = pages_seen(in, in.segs[i], c0 / group, (std::min<uint64_t>(c0 + 16 * w, n_cols) - 1) / group);
           (w == 1 ? steps16 : steps32) += p.second - p.first + 1;
         }
   }
@@ -161,7 +162,7 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
       Block b{};
       b.it.n_col = (uint32_t)std::min<uint64_t>(cols, n_cols - c0);
       const uint64_t t0 = c0 / group, t1 = (c0 + b.it.n_col - 1) / group;
-      const auto pages = pages_seen(sg, t0, t1);
+      const auto pages = pages_seen(in, sg, t0, t1);
       const uint64_t page_lo = pages.first;
       b.it.seq = (uint32_t)sg.seq;
       b.it.row0 = (uint32_t)(sg.start + t0);
@@ -462,6 +463,92 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
   return true;
 }
 
+// Segments of at least this many columns (rows x query heads of a KV head) run on the kernel for long segments.
+constexpr uint64_t PROMPT_MIN_COLS = 128;
+// A unit's fixed cost (its Q, the first tile's way through LDS, its stores) and that of a merge launch, in 64-key tiles.
+constexpr uint64_t PROMPT_UNIT_COST = 4, PROMPT_MERGE_COST = 4;
+constexpr uint64_t PROMPT_MIN_PIECE = 8;   // tiles of a key piece
+
+// Shaped scores: the units of the segments listed, a workgroup each, the longest first (the device takes them in order, so
+// the last to finish are short). A KV head's units are n_kv apart, so with 8 KV heads (or 4, or 2) those that read the same
+// pages run on one XCD (workgroup b: XCD b % 8) and share its L2. Where few long units would leave the device waiting for
+// one of them, they run as key pieces whose partials a merge combines.
+void plan_prompts(const PlanIn& in, const std::vector<uint32_t>& segs, PlanOut& o) {
+  const uint64_t group = in.n_head / in.n_kv;
+  std::vector<PrefillItem> blocks;
+  uint64_t total = 0, longest = 0;
+  for (uint32_t i : segs) {
+    const lmh_seg& sg = in.segs[i];
+    const uint64_t n_cols = sg.n * group;
+    for (uint64_t c0 = 0; c0 < n_cols; c0 += in.prompt_cols) {
+      PrefillItem it{};
+      it.n_col = (uint32_t)std::min<uint64_t>(in.prompt_cols, n_cols - c0);
+      const uint64_t t0 = c0 / group, t1 = (c0 + it.n_col - 1) / group;
+      const auto pages = pages_seen(in, sg, t0, t1);
+      it.seq = (uint32_t)sg.seq;
+      it.row0 = (uint32_t)(sg.start + t0);
+      it.pos0 = (uint32_t)(sg.pos0 + t0);
+      it.n_tok = (uint32_t)(t1 - t0 + 1);
+      it.c_off = (uint32_t)(c0 % group);
+      it.page0 = (uint32_t)pages.first;
+      it.n_pages = (uint32_t)(pages.second - pages.first + 1);
+      it.slot = NO_SLOT;
+      const uint64_t tiles = (it.n_pages + 3) / 4;
+      total += tiles + PROMPT_UNIT_COST;
+      longest = std::max(longest, tiles);
+      blocks.push_back(it);
+    }
+  }
+  total *= in.n_kv;
+  // whole units finish no sooner than the longest, or than an even share; pieces of `even` tiles with the merge
+  const uint64_t even = std::max<uint64_t>(PROMPT_MIN_PIECE, (total + in.n_cu - 1) / in.n_cu);
+  const bool cut = !in.prefill_no_split && in.hdv <= 256 && longest > even + even / 4 + PROMPT_MERGE_COST;
+  struct Piece {
+    uint32_t block, tile0, tiles, k, at;
+  };
+  std::vector<Piece> pieces;
+  for (uint32_t b = 0; b < blocks.size(); b++) {
+    const uint32_t tiles = (blocks[b].n_pages + 3) / 4;
+    const uint32_t k = cut ? (uint32_t)std::min<uint64_t>({(uint64_t)PF_MAX_PIECES, (tiles + even - 1) / even, std::max<uint64_t>(1, tiles / PROMPT_MIN_PIECE)}) : 1;
+    for (uint32_t s = 0; s < k; s++) {
+      const uint32_t a = tiles * s / k;
+      pieces.push_back(Piece{b, a, tiles * (s + 1) / k - a, k, s});
+    }
+  }
+  std::stable_sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.tiles > b.tiles; });
+  // a cut unit's slots: those of KV head 0 at base, each further KV head's after them
+  std::vector<uint32_t> base(blocks.size(), NO_SLOT);
+  uint64_t cols_cut = 0;
+  for (const Piece& p : pieces)
+    if (p.k > 1 && p.at == 0) cols_cut += blocks[p.block].n_col;
+  const uint32_t merge_heads = (uint32_t)std::max<uint64_t>(1, cols_cut * in.n_kv / 1024);
+  for (const Piece& p : pieces) {
+    if (p.k == 1 || p.at != 0) continue;
+    const PrefillItem& it = blocks[p.block];
+    base[p.block] = o.slots;
+    for (uint32_t kvh = 0; kvh < in.n_kv; kvh++) {
+      const uint32_t s0 = o.slots;
+      for_each_merge(it, group, p.k, [&](uint32_t t, uint32_t h, uint32_t nh) {
+        o.merges.push_back(MergeItem{it.row0 + t, kvh, h, s0 + t * p.k, p.k, nh});
+      }, merge_heads);
+      o.slots += it.n_tok * p.k;
+    }
+  }
+  o.prompts.reserve(pieces.size() * in.n_kv);
+  for (const Piece& p : pieces) {
+    PrefillItem it = blocks[p.block];
+    it.page0 += 4 * p.tile0;
+    it.n_pages = std::min(it.n_pages, 4 * (p.tile0 + p.tiles)) - 4 * p.tile0;
+    it.slot_stride = p.k > 1 ? p.k : 0;
+    for (uint32_t kvh = 0; kvh < in.n_kv; kvh++) {
+      it.kvh = kvh;
+      if (p.k > 1) it.slot = base[p.block] + kvh * it.n_tok * p.k + p.at;
+      o.prompts.push_back(it);
+    }
+  }
+  o.ng = (uint32_t)group;   // a piece's partial slot holds the group's heads
+}
+
 // Whole units grouped per workgroup, longest-processing-time-first: units by decreasing cost (ties
 // in list order), each to the currently least loaded workgroup (ties to the lower index). Returns
 // the largest workgroup load. The loads live in a binary min-heap of (load, workgroup) whose top
@@ -511,6 +598,24 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
   o.uwaves.clear();
   o.u_nb = o.u_w = 0;
   o.u_shared = false;
+  o.prompts.clear();
+  if (in.scored && in.prompt_cols && group <= 0xffff && in.n_kv <= 0xffff) {
+    std::vector<uint32_t> longer;
+    std::vector<lmh_seg> rest;
+    for (uint64_t i = 0; i < in.n_segs; i++) {
+      if (in.segs[i].n * group >= PROMPT_MIN_COLS) longer.push_back((uint32_t)i);
+      else if (in.segs[i].n > 0) rest.push_back(in.segs[i]);
+    }
+    if (!longer.empty()) {
+      plan_prompts(in, longer, o);
+      if (rest.empty()) return;
+      PlanIn less = in;
+      less.segs = rest.data();
+      less.n_segs = rest.size();
+      plan_units(less, o);   // every geometry with an instance above has one there
+      return;
+    }
+  }
   if (plan_units(in, o)) return;
   auto blk_at = [&](uint64_t seq, uint64_t p) {   // block id of the tile holding key p
     return (uint32_t)in.table[seq * in.bps + (((p >> 4) << 4) >> in.bt_shift)];

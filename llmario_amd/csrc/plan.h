@@ -61,6 +61,7 @@ struct PlanIn {
   uint32_t unit_waves_given = 8;    // the same where that is null
   int32_t device = 0;
   uint64_t noalloc_stage = ~0ull;   // noalloc: bytes of work list that fit the staging reserved at creation
+  uint32_t prompt_cols = 0;         // scored: columns per unit of the kernel for long segments (0: no instance)
   bool list_units = false;          // list the unit launch's units in pitems too (lmh_plan_attend)
 };
 
@@ -77,6 +78,7 @@ struct PlanOut {
   std::vector<UnitWave> uwaves;       // a unit launch (units.hip) instead of all of the above but the merges
   uint32_t u_nb = 0, u_w = 0;         // its 16-column blocks per unit and waves per workgroup
   bool u_shared = false;              // some unit is shared between waves
+  std::vector<PrefillItem> prompts;   // scored: units of long segments, a workgroup each, beside all of the above
 };
 
 // Segments of at least this many rows run on the matrix-core prefill kernel by default (Metal's

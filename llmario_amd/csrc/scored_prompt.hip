@@ -1,0 +1,567 @@
+// scored_prompt.hip — attention with shaped scores (lmh_attend_scored) of long segments on gfx950 matrix cores.
+//
+// A unit is up to 8 * COLS columns (token, query head) of one segment and KV head, flattened token-major as
+// units.hip's, over the key pages its columns see; one workgroup of 8 waves (two per SIMD) takes a unit, wave w its
+// columns COLS * w .. (COLS: 32 as two 16-column blocks; 16 on 256-wide heads). The workgroup walks 64-key tiles:
+// all its waves share each tile's K and V through LDS, so pages are read once per unit and expanded once:
+//   f16: as they are. bf16: widened to f16. q8_0: code * scale as f16 hi + lo parts (exact: 7 + 11 bits).
+//   S^T[keys x cols] = K . Q^T       v_mfma_f32_16x16x32_f16, Q as f16 hi + lo parts of the column scaled by a
+//                                    power of two to below 1 (22 bits of its largest element)
+//   O^T[dims x cols] += V^T . P^T    v_mfma_f32_16x16x32_f16, weights as f16 hi + lo parts
+// (q8_0: K hi . Q hi + K hi . Q lo + K lo . Q hi, and V likewise.) f16 has less range than bf16 or a scaled code: K
+// and V are scaled by powers of two taken from the largest magnitude of the unit's first tile when that lies outside
+// 2^-6 .. 2^8, and a unit whose K leaves f16's range later, or whose outputs are not finite (a NaN or an infinity in
+// V, seen or not), is computed again on the vector units in f32 (redo), straight from the pages.
+//
+// Per tile: the next tile's pages are requested into registers, the tile in LDS is multiplied, then the registers are
+// expanded into the other LDS buffer and one barrier publishes it.
+#include "decode_tile.h"
+#include "score.h"
+
+namespace lmh {
+namespace {
+
+using namespace dtile;
+
+constexpr int PW = 8, NTH = 64 * PW, BK = 64;
+
+template <int KVT, int HD>
+struct Shape {
+  static constexpr bool Q8 = KVT == KV_Q8, BF = KVT == KV_BF16;
+  static constexpr int NCB = HD <= 128 ? 2 : 1, COLS = 16 * NCB;
+  static constexpr int NC = HD / 32, NJ = HD / 16;
+  static constexpr int SIDE = BK * HD * 2;                  // bytes of a tile's K or V part in LDS
+  static constexpr int PARTS = Q8 ? 2 : 1;
+  static constexpr int STAGE = 2 * SIDE * PARTS;            // [K hi][K lo][V hi][V lo]
+  static constexpr int LDS = 2 * STAGE + 128;               // .. and the workgroup's words
+  static constexpr int NI = HD == 64 ? 1 : Q8 ? HD / 64 : NC / 2;   // staged items per wave and tile
+  static constexpr int ROWS_I = Q8 ? 1 : 2;                 // 1 KiB page rows of an item
+};
+
+// One f32 value of key m, dim d of a tile-layout page (K or V) of head base `head`, tile `sub` of the block.
+template <int KVT>
+__device__ inline float page_value(const uint8_t* head, uint32_t sub, uint32_t tile, uint32_t scale, uint32_t tile_s, bool is_v, uint32_t m,
+                                   uint32_t d, uint32_t hd) {
+  const uint8_t* t = head + (size_t)sub * tile;
+  if constexpr (KVT == KV_Q8) {
+    const float c = (float)*(const int8_t*)(t + (is_v ? vq8_off(m, d) : kq8_off(m, d)));
+    return c * h_to_f(*(const uint16_t*)(head + scale + (size_t)sub * tile_s + (m * (hd / 32) + d / 32) * 2));
+  } else {
+    const uint16_t b = *(const uint16_t*)(t + (is_v ? v16_off(m, d) : k16_off(m, d)));
+    return KVT == KV_F16 ? h_to_f(b) : __uint_as_float((uint32_t)b << 16);
+  }
+}
+
+// Column (row, head) of a unit in f32 from the pages, one wave: lanes over keys for the scores, over dims for the sums.
+// out: the row's HD values, or its partial (raw sums, then reference and sum).
+template <int KVT, int HD>
+__device__ __noinline__ void redo(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, uint32_t seq, uint32_t kvh, uint32_t head,
+                                  uint32_t pos, uint32_t first, uint32_t end, const float* q, float* out, bool partial) {
+  constexpr int ND = HD / 64;
+  const uint32_t lane = threadIdx.x & 63u, bt_mask = (1u << g.bt_shift) - 1u;
+  const int32_t* tab = g.table + (size_t)seq * g.bps;
+  float m = -INFINITY, l = 0.f, o[ND];
+  for (int i = 0; i < ND; i++) o[i] = 0.f;
+  const float slope = sc.slopes ? sc.slopes[head] * LOG2E : 0.f;
+  for (uint32_t k0 = first; k0 < end; k0 += 64) {
+    const uint32_t key = min(k0 + lane, end - 1), n = min(64u, end - k0);
+    const uint8_t* b = g.pool + (size_t)(uint32_t)tab[key >> g.bt_shift] * g.block_bytes;
+    const uint8_t* kh = b + g.k_off + (size_t)kvh * g.k_head;
+    float s = 0.f;
+    for (uint32_t d = 0; d < (uint32_t)HD; d++)
+      s = fmaf(q[d], page_value<KVT>(kh, (key & bt_mask) >> 4, g.k_tile, g.k_scale, g.k_tile_s, false, key & 15u, d, HD), s);
+    float p[1] = {s * u.scale_log2};
+    if (sc.cap_log2 > 0.f) cap_scores<1>(p, sc.cap_log2);
+    if (sc.slopes) bias_scores<1>(p, slope, (float)(int)(key - pos), [](int) { return 0.f; });
+    if (lane >= n) p[0] = -INFINITY;
+    float mn = fmaxf(m, p[0]);
+    for (int x = 32; x >= 1; x >>= 1) mn = fmaxf(mn, __shfl_xor(mn, x));
+    const float ref = mn == -INFINITY ? 0.f : mn, alpha = exp2_fast(m - ref), w = lane < n ? exp2_fast(p[0] - ref) : 0.f;
+    float sum = w;
+    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+    l = l * alpha + sum;
+    m = mn;
+    for (int i = 0; i < ND; i++) o[i] *= alpha;
+    for (uint32_t j = 0; j < n; j++) {
+      const uint32_t kj = k0 + j;
+      const float wj = __shfl(w, (int)j);
+      const uint8_t* vh = g.pool + (size_t)(uint32_t)tab[kj >> g.bt_shift] * g.block_bytes + g.v_off + (size_t)kvh * g.v_head;
+      for (int i = 0; i < ND; i++)
+        o[i] = fmaf(wj, page_value<KVT>(vh, (kj & bt_mask) >> 4, g.v_tile, g.v_scale, g.v_tile_s, true, kj & 15u, lane + 64 * i, HD), o[i]);
+    }
+  }
+  const float mul = partial ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+  for (int i = 0; i < ND; i++) out[lane + 64 * i] = o[i] * mul;
+  if (partial && lane == 0) {
+    out[HD] = m;
+    out[HD + 1] = l;
+  }
+}
+
+template <int KVT, int HD>
+__global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillItem* items, const float* q, float* out, MergeCopy mc) {
+  using C = Shape<KVT, HD>;
+  constexpr bool Q8 = C::Q8, BF = C::BF;
+  constexpr int NCB = C::NCB, COLS = C::COLS, NC = C::NC, NJ = C::NJ, NI = C::NI;
+  extern __shared__ __attribute__((aligned(16))) uint8_t prompt_lds[];
+  uint32_t* words = (uint32_t*)(prompt_lds + 2 * C::STAGE);   // [8] K maxima, [8] V maxima, [16] the redo flag
+  copy_merges(mc, blockIdx.x, gridDim.x);
+  const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t hq = lane & 15u, grp = lane >> 4, G = u.group;
+  // the unit's record: one load, a word per lane, broadcast to scalar registers
+  const uint32_t word = lane < sizeof(PrefillItem) / 4 ? ((const uint32_t*)(items + blockIdx.x))[lane] : 0u;
+  auto fld = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)word, i); };
+  const uint32_t seq = fld(0), kvh = fld(1), row0 = fld(2), pos0 = fld(3), c_off = fld(5), n_col = fld(6), page0 = fld(7),
+                 n_pages = fld(8), slot = fld(9), stride = fld(10);
+  const uint32_t page_end = page0 + n_pages, n_tiles = (n_pages + 3) / 4;
+
+  // ---- page tiles of a staged item: item i of wave w is a K item (two chunk rows of a page tile; q8_0: a row of codes)
+  // or a V item (the same dim row of page tiles 2h and 2h + 1, the two of half h; q8_0: a row of codes of one)
+  auto is_k = [&](int i) -> bool { return HD == 64 ? w < 4 : i < NI / 2; };
+  auto index = [&](int i) -> uint32_t { return HD == 64 ? w & 3u : w + 8u * (i % (NI / 2 ? NI / 2 : 1)); };
+  // the page tiles (0 .. 3 of the 64-key tile) an item reads, and its row there
+  auto tile_of = [&](int i, int r) -> uint32_t {
+    const uint32_t x = index(i);
+    if constexpr (Q8) return x / (HD / 64);
+    return is_k(i) ? x / (NC / 2) : 2 * (x / NC) + r;
+  };
+  auto row_of = [&](int i, int r) -> uint32_t {
+    const uint32_t x = index(i);
+    if constexpr (Q8) return x % (HD / 64);
+    return is_k(i) ? x % (NC / 2) * 2 + r : x % NC;
+  };
+  typedef const __attribute__((address_space(4))) int32_t cint;
+  cint* tab = (cint*)(uintptr_t)(g.table + (size_t)seq * g.bps);
+  const uint32_t bt_mask = (1u << g.bt_shift) - 1u;
+  int blk[NI][C::ROWS_I];
+  auto page_of = [&](uint32_t t, int i, int r) -> uint32_t { return min(page0 + 4 * t + tile_of(i, r), page_end - 1); };
+  auto ids = [&](uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+#pragma unroll
+      for (int r = 0; r < C::ROWS_I; r++) blk[i][r] = tab[(page_of(t, i, r) << 4) >> g.bt_shift];
+  };
+  uint4 raw[NI][C::ROWS_I];
+  uint32_t rs[NI][Q8 ? 4 : 1];   // q8_0: the scales (K: the key's two chunks; V: of four keys)
+  auto request = [&](uint32_t t) {   // with the block ids of tile t
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const bool k = is_k(i);
+#pragma unroll
+      for (int r = 0; r < C::ROWS_I; r++) {
+        const uint32_t sub = ((page_of(t, i, r) << 4) & bt_mask) >> 4;
+        const uint8_t* head = g.pool + (size_t)(uint32_t)blk[i][r] * g.block_bytes + (k ? g.k_off + (size_t)kvh * g.k_head : g.v_off + (size_t)kvh * g.v_head);
+        raw[i][r] = *(const uint4*)(head + (size_t)sub * (k ? g.k_tile : g.v_tile) + row_of(i, r) * 1024 + lane * 16);
+        if constexpr (Q8) {
+          const uint8_t* s = head + (k ? g.k_scale : g.v_scale) + (size_t)sub * (k ? g.k_tile_s : g.v_tile_s) + row_of(i, r) * 4;
+          if (k) rs[i][0] = *(const uint32_t*)(s + hq * (2 * NC));
+          else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) rs[i][e] = *(const uint32_t*)(s + (4 * grp + e) * (2 * NC));
+          }
+        }
+      }
+    }
+  };
+  ids(0);
+  request(0);
+  ids(1);
+
+  // ---- Q of the wave's columns (the B operand of S^T = K Q^T), while the first tile is on its way
+  uint32_t ct[NCB], ch[NCB], clo[NCB], cend[NCB], cpos[NCB];
+  bool cv[NCB];
+  float slope[NCB], qscale[NCB];
+  uint32_t lo_max = 0, end_min = ~0u, lo_min = ~0u, end_max = 0;
+  bool any = false;
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    const uint32_t c = w * COLS + 16 * x + hq;
+    cv[x] = c < n_col;
+    ct[x] = cv[x] ? (c + c_off) / G : 0;
+    ch[x] = cv[x] ? (c + c_off) - ct[x] * G : 0;
+    cpos[x] = pos0 + ct[x];
+    clo[x] = (u.window > 0 && cpos[x] + 1 > u.window) ? cpos[x] + 1 - u.window : 0;
+    cend[x] = cpos[x];
+    if (sc.ranges) {
+      const uint2 r = sc.ranges[row0 + ct[x]];
+      clo[x] = r.x;
+      cend[x] = r.y;
+    }
+    slope[x] = sc.slopes && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
+    if (cv[x]) {
+      lo_max = max(lo_max, clo[x]);
+      end_min = min(end_min, cend[x]);
+      if (clo[x] <= cend[x]) {
+        lo_min = min(lo_min, clo[x]);
+        end_max = max(end_max, cend[x]);
+        any = true;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 1; i < 16; i <<= 1) {
+    lo_max = max(lo_max, (uint32_t)__shfl_xor((int)lo_max, i));
+    end_min = min(end_min, (uint32_t)__shfl_xor((int)end_min, i));
+    lo_min = min(lo_min, (uint32_t)__shfl_xor((int)lo_min, i));
+    end_max = max(end_max, (uint32_t)__shfl_xor((int)end_max, i));
+  }
+  lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+  end_min = __builtin_amdgcn_readfirstlane(end_min);
+  lo_min = __builtin_amdgcn_readfirstlane(lo_min);     // no column of the wave sees a key outside lo_min .. end_max
+  end_max = __builtin_amdgcn_readfirstlane(end_max);
+  any = __ballot(any) != 0;
+  h8 qp[2][NCB][NC];
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    const float* qrow = q + ((size_t)(row0 + ct[x]) * u.n_head + (size_t)kvh * G + ch[x]) * HD;
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+    f4 v[NC][2];
+    float am = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) v[c][e] = cv[x] ? *(const f4u*)(qrow + 32 * c + 8 * grp + 4 * e) : f4u{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(v[c][i >> 2][i & 3]));
+    }
+    const int e = __builtin_amdgcn_frexp_expf(xmax_groups(am));
+    qscale[x] = ldexpf(u.scale_log2, e);
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float y = ldexpf(v[c][i >> 2][i & 3], -e);
+        const _Float16 hi = (_Float16)y;
+        qp[0][x][c][i] = hi;
+        qp[1][x][c][i] = (_Float16)(y - (float)hi);
+      }
+  }
+
+  // ---- the powers of two of K and V (bf16, q8_0), from the first tile
+  float k_mul = 1.f, v_mul = 1.f;
+  int v_exp = 0;
+  if (threadIdx.x == 0) words[16] = 0;
+  if constexpr (BF || Q8) {
+    uint32_t top[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      uint32_t t = 0;
+      auto see = [&](uint32_t x) { t = max(t, max(x & 0x7fffu, (x >> 16) & 0x7fffu)); };
+      if constexpr (Q8) {
+        see(rs[i][0]);
+        if (!is_k(i)) {
+          see(rs[i][1]);
+          see(rs[i][2]);
+          see(rs[i][3]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          see(raw[i][r].x);
+          see(raw[i][r].y);
+          see(raw[i][r].z);
+          see(raw[i][r].w);
+        }
+      }
+      if (is_k(i)) top[0] = max(top[0], t);
+      else top[1] = max(top[1], t);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], x));
+      top[1] = max(top[1], (uint32_t)__shfl_xor((int)top[1], x));
+    }
+    if (lane == 0) {
+      words[w] = top[0];
+      words[8 + w] = top[1];
+    }
+    __syncthreads();
+    uint32_t km = 0, vm = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      km = max(km, words[i]);
+      vm = max(vm, words[8 + i]);
+    }
+    auto exponent = [&](uint32_t bits) -> int {   // of the largest value: in [2^(e-1), 2^e); 0 in the usual range
+      const float f = Q8 ? h_to_f((uint16_t)bits) * 127.0f : __uint_as_float(bits << 16);
+      if (!(f < INFINITY) || f == 0.f) return 0;
+      const int e = __builtin_amdgcn_frexp_expf(f);
+      return e >= -6 && e <= 8 ? 0 : min(max(e, -120), 120);
+    };
+    const int ke = __builtin_amdgcn_readfirstlane(exponent(km));
+    v_exp = __builtin_amdgcn_readfirstlane(exponent(vm));
+    k_mul = ldexpf(1.0f, -ke);
+    v_mul = ldexpf(1.0f, -v_exp);
+#pragma unroll
+    for (int x = 0; x < NCB; x++) qscale[x] = ldexpf(qscale[x], ke);
+  }
+
+  // ---- registers into an LDS buffer
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  u16x2 k_top = 0;   // largest |K| bits written by this lane (bf16, q8_0): 0x7c00 and more left f16's range
+  auto widen = [&](uint32_t x, float mul) -> uint32_t {   // two bf16
+    const f2 y = f2{__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)} * mul;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(y, h2));
+  };
+  auto widen4 = [&](uint4 x, float mul) -> uint4 { return make_uint4(widen(x.x, mul), widen(x.y, mul), widen(x.z, mul), widen(x.w, mul)); };
+  auto note = [&](uint32_t x) { k_top = __builtin_elementwise_max(k_top, __builtin_bit_cast(u16x2, x & 0x7fff7fffu)); };
+  // two codes times their scales as hi and lo parts
+  auto expand = [&](float a, float b, uint32_t& hi, uint32_t& lo) { split_pair(a, b, hi, lo); };
+  auto write = [&](uint32_t buf) {
+    uint8_t* st = prompt_lds + buf * C::STAGE;
+    uint8_t* const kst = st;
+    uint8_t* const vst = st + C::PARTS * C::SIDE;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      if constexpr (Q8) {
+        const uint32_t t = tile_of(i, 0), r = row_of(i, 0);
+        const uint32_t* cw = (const uint32_t*)&raw[i][0];
+        if (is_k(i)) {   // codes 0 .. 7: chunk 2r of key hq, 8 .. 15: chunk 2r + 1
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const float s = h_to_f((uint16_t)(c ? rs[i][0] >> 16 : rs[i][0])) * k_mul;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t x = cw[2 * c + (e >> 1)] >> (16 * (e & 1));
+              expand((float)(int8_t)x * s, (float)(int8_t)(x >> 8) * s, hi[e], lo[e]);
+              note(hi[e]);
+            }
+            uint8_t* at = kst + (t * NC + 2 * r + c) * 1024 + lane * 16;
+            *(uint4*)at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *(uint4*)(at + C::SIDE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        } else {         // word j: dims block 4r + j, keys 4 grp .. + 3
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float s[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = h_to_f((uint16_t)(j >> 1 ? rs[i][e] >> 16 : rs[i][e])) * v_mul;
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const uint32_t x = cw[j] >> (16 * e);
+              expand((float)(int8_t)x * s[2 * e], (float)(int8_t)(x >> 8) * s[2 * e + 1], hi[e], lo[e]);
+            }
+            uint8_t* at = vst + ((t >> 1) * NJ + 4 * r + j) * 1024 + lane * 16 + (t & 1) * 8;
+            *(uint2*)at = make_uint2(hi[0], hi[1]);
+            *(uint2*)(at + C::SIDE) = make_uint2(lo[0], lo[1]);
+          }
+        }
+      } else if (is_k(i)) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          uint4 x = raw[i][r];
+          if constexpr (BF) {
+            x = widen4(x, k_mul);
+            note(x.x);
+            note(x.y);
+            note(x.z);
+            note(x.w);
+          }
+          *(uint4*)(kst + (tile_of(i, r) * NC + row_of(i, r)) * 1024 + lane * 16) = x;
+        }
+      } else {           // [4 keys of dim d | of dim d + 16] of both tiles into blocks 2b and 2b + 1 of 8 keys
+        uint4 a = raw[i][0], b = raw[i][1];
+        if constexpr (BF) {
+          a = widen4(a, v_mul);
+          b = widen4(b, v_mul);
+        }
+        uint8_t* at = vst + ((tile_of(i, 0) >> 1) * NJ + 2 * row_of(i, 0)) * 1024 + lane * 16;
+        *(uint4*)at = make_uint4(a.x, a.y, b.x, b.y);
+        *(uint4*)(at + 1024) = make_uint4(a.z, a.w, b.z, b.w);
+      }
+    }
+  };
+  write(0);
+  __syncthreads();
+
+  // ---- the walk
+  constexpr float UP = 7.0f;   // weights are taken against m - 7 (up to 2^15 with the lazy reference): more of them in f16's range
+  float m[NCB], lsum[NCB];
+  f4 O[NCB][NJ];
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    m[x] = -INFINITY;
+    lsum[x] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) O[x][j] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma clang loop unroll(disable)
+  for (uint32_t t = 0; t < n_tiles; t++) {
+    if (t + 1 < n_tiles) {
+      request(t + 1);
+      ids(t + 2);
+    }
+    const uint8_t* st = prompt_lds + (t & 1) * C::STAGE + lane * 16;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t key0 = ((page0 + 4 * t) << 4) + 32 * h;
+      if (!any || key0 > end_max || key0 + 31 < lo_min || key0 >= page_end << 4) continue;   // uniform over the wave
+      f4 s[NCB][2];
+#pragma unroll
+      for (int x = 0; x < NCB; x++) s[x][0] = s[x][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+          const uint8_t* at = st + ((2 * h + kk) * NC + c) * 1024;
+          const h8 kc = *(const h8*)at;
+#pragma unroll
+          for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qp[0][x][c], s[x][kk], 0, 0, 0);
+#pragma unroll
+          for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qp[1][x][c], s[x][kk], 0, 0, 0);
+          if constexpr (Q8) {
+            const h8 kl = *(const h8*)(at + C::SIDE);
+#pragma unroll
+            for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qp[0][x][c], s[x][kk], 0, 0, 0);
+          }
+        }
+      const bool need_mask = key0 + 31 > end_min || key0 < lo_max || key0 + 32 > page_end << 4;
+      h8 ph[NCB], pl[NCB];
+#pragma unroll
+      for (int x = 0; x < NCB; x++) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = s[x][i >> 2][i & 3] * qscale[x];
+        if (sc.cap_log2 > 0.f) cap_scores<8>(p, sc.cap_log2);
+        if (sc.slopes) bias_scores<8>(p, slope[x], (float)(int)(key0 + 4 * grp - cpos[x]), [](int i) { return (float)(16 * (i >> 2) + (i & 3)); });
+        if (need_mask) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint32_t key = key0 + 16 * (i >> 2) + 4 * grp + (i & 3);
+            if (key > cend[x] || key < clo[x] || key >= page_end << 4) p[i] = -INFINITY;
+          }
+        }
+        float lm = p[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) lm = fmaxf(lm, p[i]);
+        if (__ballot(lm > m[x] + 8.0f)) {
+          const float tm = xmax_groups(lm);
+          const float mn = tm > m[x] + 8.0f ? tm : m[x];
+          const float alpha = mn == m[x] ? 1.f : (m[x] == -INFINITY ? 0.f : exp2_fast(m[x] - mn));
+          lsum[x] *= alpha;
+#pragma unroll
+          for (int j = 0; j < NJ; j++) O[x][j] *= alpha;
+          m[x] = mn;
+        }
+        const float mref = m[x] == -INFINITY ? 0.f : m[x] - UP;   // every score is -inf while m is
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = exp2_fast(p[i] - mref);
+        lsum[x] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        uint32_t hw[4], lw[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_pair(p[2 * i], p[2 * i + 1], hw[i], lw[i]);
+        ph[x] = __builtin_bit_cast(h8, make_uint4(hw[0], hw[1], hw[2], hw[3]));
+        pl[x] = __builtin_bit_cast(h8, make_uint4(lw[0], lw[1], lw[2], lw[3]));
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        const uint8_t* at = st + C::PARTS * C::SIDE + (h * NJ + j) * 1024;
+        const h8 va = *(const h8*)at;
+#pragma unroll
+        for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[x], O[x][j], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[x], O[x][j], 0, 0, 0);
+        if constexpr (Q8) {
+          const h8 vl = *(const h8*)(at + C::SIDE);
+#pragma unroll
+          for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[x], O[x][j], 0, 0, 0);
+        }
+      }
+    }
+    if (t + 1 < n_tiles) write((t + 1) & 1);
+    __syncthreads();
+  }
+
+  // ---- results
+  if constexpr (BF || Q8) {
+    if (max(k_top[0], k_top[1]) >= 0x7c00) words[16] = 1;
+    __syncthreads();
+  }
+  bool bad = (BF || Q8) && words[16] != 0;
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    lsum[x] = xsum_groups(lsum[x]);
+    float z = lsum[x];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) z += (O[x][j][0] + O[x][j][1]) + (O[x][j][2] + O[x][j][3]);
+    bad |= cv[x] && !__builtin_isfinite(z);
+  }
+  auto row_at = [&](uint32_t tok, uint32_t head) -> float* {
+    if (slot == NO_SLOT) return out + ((size_t)(row0 + tok) * u.n_head + (size_t)kvh * G + head) * HD;
+    return u.part + ((size_t)(slot + tok * stride) * u.ng + head) * (HD + 4);
+  };
+  if (__builtin_expect(__ballot(bad) != 0, 0)) {
+    for (uint32_t c = 0; c < (uint32_t)COLS && w * COLS + c < n_col; c++) {
+      const uint32_t a = w * COLS + c + c_off, tok = a / G, head = a - tok * G, pos = pos0 + tok;
+      uint32_t first = (u.window > 0 && pos + 1 > u.window) ? pos + 1 - u.window : 0, last = pos;
+      if (sc.ranges) {
+        const uint2 r = sc.ranges[row0 + tok];
+        first = r.x;
+        last = r.y;
+      }
+      first = max(first, page0 << 4);
+      const uint32_t end = first > last ? first : min(last + 1, page_end << 4);   // (end <= first: it sees nothing here)
+      redo<KVT, HD>(g, u, sc, seq, kvh, kvh * G + head, pos, first, end,
+                    q + ((size_t)(row0 + tok) * u.n_head + (size_t)kvh * G + head) * HD, row_at(tok, head), slot != NO_SLOT);
+    }
+    return;
+  }
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    if (!cv[x]) continue;
+    float* op = row_at(ct[x], ch[x]);
+    const float mul = (slot != NO_SLOT ? 1.0f : lsum[x] == 0.f ? 0.f : 1.0f / lsum[x]) * ldexpf(1.0f, v_exp);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const f4 o = O[x][j] * mul;
+      *(f4u*)(op + 16 * j + 4 * grp) = f4u{o[0], o[1], o[2], o[3]};
+    }
+    if (slot != NO_SLOT && grp == 0) {
+      op[HD] = m[x] - UP;   // the reference the weights were taken against
+      op[HD + 1] = lsum[x];
+    }
+  }
+}
+
+// f(type, width) of the instance that takes a geometry; false: none does.
+template <typename Fn>
+bool with_prompt(uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout, Fn&& f) {
+  if (layout != LAYOUT_TILES || hd != hdv) return false;
+#define LMH_P(T, H)                                                                              \
+  if (kv_type == T && hd == H) {                                                                 \
+    f(std::integral_constant<uint32_t, T>{}, std::integral_constant<int, H>{});                  \
+    return true;                                                                                 \
+  }
+  LMH_P(KV_F16, 64) LMH_P(KV_F16, 128) LMH_P(KV_F16, 256) LMH_P(KV_BF16, 64) LMH_P(KV_BF16, 128) LMH_P(KV_BF16, 256)
+  LMH_P(KV_Q8, 64) LMH_P(KV_Q8, 128)
+#undef LMH_P
+  return false;
+}
+
+}  // namespace
+
+uint32_t scored_prompt_cols(uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout) {
+  uint32_t n = 0;
+  with_prompt(kv_type, hd, hdv, layout, [&](auto t, auto h) { n = PW * Shape<decltype(t)::value, decltype(h)::value>::COLS; });
+  return n;
+}
+
+hipError_t launch_scored_prompts(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, const PrefillItem* items, uint32_t n_items,
+                                 const float* q, float* out, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev) {
+  if (n_items == 0) return hipSuccess;
+  hipError_t e = hipErrorInvalidValue;
+  with_prompt(g.kv_type, g.hd, g.hdv, g.layout, [&](auto t, auto h) {
+    constexpr int T = decltype(t)::value, H = decltype(h)::value;
+    LMH_LAUNCH(ev, (scored_prompt_kernel<T, H>), dim3(n_items), dim3(NTH), (Shape<T, H>::LDS), s, g, u, sc, items, q, out, mc);
+    e = hipGetLastError();
+  });
+  return e;
+}
+
+}  // namespace lmh

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "decode_tile.h"
+#include "score.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -83,6 +84,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
                                           float* out, float* lds, const ScoreGeom& sc = ScoreGeom{}) {
   using C = Cfg<F, HDP, HDVP, NB, SC>;
   constexpr bool BF = C::BF, Q8 = C::Q8, ROWS = C::ROWS, F32 = C::F32;
+  constexpr bool B3 = F == FR_BF16 || (SC && F == FT_BF16);   // P.V in bf16, whose range V may use
   constexpr int KT = C::KT, NC = C::NC, NJ = C::NJ, GRP = C::GRP, NCH = HDVP / 32;
   using MT = typename std::conditional<BF, b8, h8>::type;
   const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -123,7 +125,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
       clo[x] = (u.window > 0 && cend[x] + 1 > u.window) ? cend[x] + 1 - u.window : 0;
       if constexpr (SC) {
         cpos[x] = cend[x];
-        slope[x] = sc.slopes && cv[x] ? sc.slopes[kvh * G + ch[x]] * 1.4426950408889634f : 0.f;
+        slope[x] = sc.slopes && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
       }
     }
     if (SC && sc.ranges) {
@@ -274,7 +276,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
           raw[c][0] = on ? *(const f4u*)(qrow + d) : f4u{0.f, 0.f, 0.f, 0.f};
           raw[c][1] = on ? *(const f4u*)(qrow + d + 4) : f4u{0.f, 0.f, 0.f, 0.f};
         }
-        if constexpr (F == FR_F16) {
+        if constexpr (F == FR_F16 || (SC && !BF)) {   // (shaped scores: f16 parts of a Q far from 1 too)
           float am = 0.f;
 #pragma unroll
           for (int c = 0; c < NC; c++)
@@ -322,7 +324,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
     // column's own keys: the largest scale of the first step in which it sees one. Where the products are
     // in f32's range, 0, and the weights times 2^-8 (of every wave and piece alike): none is over 1, so no
     // weighted V leaves it. (A shift in the exponent would cost its argument the bits it grows by.)
-    constexpr bool UNIT_P = F32 || F == FR_BF16;
+    constexpr bool UNIT_P = F32 || B3;
     // 16-bit rows: O that is not finite makes the unit run again with every step's V tested.
     constexpr bool AGAIN = Q8 || (ROWS && !F32);
     bool checked = false;
@@ -439,15 +441,9 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
 #pragma unroll
             for (int r = 0; r < 4; r++) p[x][4 * kk + r] = s[x][kk][r] * qscale[x];
           if constexpr (SC) {
-            if (sc.cap_log2 > 0.f) {   // (qscale: scale / cap)
-#pragma unroll
-              for (int i = 0; i < 4 * KT; i++) p[x][i] = sc.cap_log2 * tanhf(p[x][i]);
-            }
-            if (sc.slopes) {
-              const float d0 = (float)(int)(key0 + 4 * grp - cpos[x]);
-#pragma unroll
-              for (int i = 0; i < 4 * KT; i++) p[x][i] = fmaf(-slope[x], fabsf(d0 + (float)(16 * (i >> 2) + (i & 3))), p[x][i]);
-            }
+            if (sc.cap_log2 > 0.f) cap_scores<4 * KT>(p[x], sc.cap_log2);   // (qscale: scale / cap)
+            if (sc.slopes)
+              bias_scores<4 * KT>(p[x], slope[x], (float)(int)(key0 + 4 * grp - cpos[x]), [](int i) { return (float)(16 * (i >> 2) + (i & 3)); });
           }
           if (need_mask) {
 #pragma unroll
@@ -581,7 +577,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
         bool bad_v = false;
         auto nonfinite = [](uint32_t v) -> uint32_t {   // mask of the word's non-finite values
           if constexpr (F32) return (v & 0x7f800000u) == 0x7f800000u ? ~0u : 0u;
-          constexpr uint32_t E = F == FT_BF16 ? 0x4780u : BF ? 0x7f80u : 0x7c00u;   // the least non-finite magnitude
+          constexpr uint32_t E = F == FT_BF16 && !B3 ? 0x4780u : BF ? 0x7f80u : 0x7c00u;   // the least non-finite magnitude
           return ((v & 0x7fffu) >= E ? 0xffffu : 0u) | ((v & 0x7fff0000u) >= E << 16 ? 0xffff0000u : 0u);
         };
         if constexpr (!Q8) {
@@ -669,15 +665,15 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
         } else {
           // P as f16 hi + lo parts on V in f16 (bf16 tiles widened), or in the row layout as three parts of
           // the pages' type on V as it is
-          constexpr int PP = ROWS ? 3 : 2;
-          using PT = typename std::conditional<F == FR_BF16, b8, h8>::type;
+          constexpr int PP = ROWS || B3 ? 3 : 2;
+          using PT = typename std::conditional<B3, b8, h8>::type;
           PT pp[PP][NB];
 #pragma unroll
           for (int x = 0; x < NB; x++) {
             uint32_t pw[PP][4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              if constexpr (F == FR_BF16) {
+              if constexpr (B3) {
                 typedef float f2 __attribute__((ext_vector_type(2)));
                 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
                 f2 r = {p[x][2 * i], p[x][2 * i + 1]};
@@ -726,7 +722,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
               wv[2] = w1[o];
               wv[3] = w1[o + 1];
             }
-            if constexpr (F == FT_BF16) {
+            if constexpr (F == FT_BF16 && !B3) {
 #pragma unroll
               for (int i = 0; i < 4; i++) wv[i] = bf2_h2(wv[i]);
             }
@@ -735,7 +731,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
             for (int k = 0; k < PP; k++)
 #pragma unroll
               for (int x = 0; x < NB; x++) {
-                if constexpr (F == FR_BF16) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[k][x], O[x][j], 0, 0, 0);
+                if constexpr (B3) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[k][x], O[x][j], 0, 0, 0);
                 else O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pp[k][x], O[x][j], 0, 0, 0);
               }
             if constexpr (!ROWS) {
@@ -762,7 +758,7 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
                 else seeh[x][i] = on ? (_Float16)1.0f : (_Float16)0.0f;
               }
             auto kind = [](float v, int k) -> float {   // k: 0 +inf, 1 -inf, 2 NaN
-              constexpr float TOP = F == FT_BF16 ? 65536.f : INFINITY;
+              constexpr float TOP = F == FT_BF16 && !B3 ? 65536.f : INFINITY;
               return (k == 2 ? v != v : k == 0 ? v >= TOP : v <= -TOP) ? 1.0f : 0.0f;
             };
 #pragma unroll

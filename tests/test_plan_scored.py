@@ -23,16 +23,18 @@ def scored_plan(kv, geo, bt, table, segs, lo, hi, window=0, n_cu=256, per_cu=8, 
     r = RowRanges(lo, hi)
     lo_p = C.cast(r.lo, C.c_void_p) if r.lo is not None else None
     hi_p = C.cast(r.hi, C.c_void_p) if r.hi is not None else None
-    c, n_items = N.PlanWaveCounts(), N.u64()
-    rc = N.lib().lmh_plan_scored(C.byref(d), arr, len(segs), lo_p, hi_p, per_cu, None, 0, None, 0, None, 0, C.byref(c), C.byref(n_items))
-    if rc != N.OK and not (c.n_waves or n_items.value):
-        return rc, None, None, None, c
+    c, n_items, n_prompts = N.PlanWaveCounts(), N.u64(), N.u64()
+    counts = (C.byref(c), C.byref(n_items), C.byref(n_prompts))
+    rc = N.lib().lmh_plan_scored(C.byref(d), arr, len(segs), lo_p, hi_p, per_cu, None, 0, None, 0, None, 0, None, 0, *counts)
+    if rc != N.OK and not (c.n_waves or n_items.value or n_prompts.value):
+        return rc, None, None, None, None, c
     waves, items = np.zeros((c.n_waves, 10), np.uint32), np.zeros((n_items.value, 8), np.uint32)
+    prompts = np.zeros((n_prompts.value, 20), np.uint32)
     merges = np.zeros((c.n_merges, 6), np.uint32)
     at = lambda a: a.ctypes.data_as(C.c_void_p)
     rc = N.lib().lmh_plan_scored(C.byref(d), arr, len(segs), lo_p, hi_p, per_cu, at(waves), len(waves), at(items), len(items),
-                                 at(merges), len(merges), C.byref(c), C.byref(n_items))
-    return rc, waves, items, merges, c
+                                 at(prompts), len(prompts), at(merges), len(merges), *counts)
+    return rc, waves, items, prompts, merges, c
 
 
 def seen(segs, lo, hi, window):
@@ -46,14 +48,14 @@ def seen(segs, lo, hi, window):
     return out
 
 
-def check(kv, geo, bt, table, segs, lo, hi, window, waves, items, merges, c):
+def check(kv, geo, bt, table, segs, lo, hi, window, waves, items, prompts, merges, c):
     n_head, n_kv, _, _ = geo
     group, rows = n_head // n_kv, seen(segs, lo, hi, window)
     step = 1 if kv == "f32" else 2
     pages = {}     # (row, head) -> pages its unit's waves walk
     slots = {}     # (row, head) -> slots its pieces leave
     W, at = c.waves_per_wg, 0
-    assert not (len(waves) and len(items)) and (len(waves) == 0 or len(waves) % W == 0)
+    assert not (len(waves) + len(prompts) and len(items)) and (len(waves) == 0 or len(waves) % W == 0)
     while at < len(waves):
         seq, row0, pos0, page0, _, slot, _, _, head, cols = (int(x) for x in waves[at])
         n = cols >> 16 & 0xFF
@@ -80,6 +82,19 @@ def check(kv, geo, bt, table, segs, lo, hi, window, waves, items, merges, c):
                 assert slot + (col // group) * k < c.slots
                 slots.setdefault((t, h), []).append(slot + (col // group) * k)
         at += n
+    cols = 128 if geo[2] == 256 else 256
+    assert all(int(a[8]) + 3 >= int(b[8]) for a, b in zip(prompts, prompts[1:]))   # the longest first (in 64-key tiles)
+    for u in prompts:
+        seq, kvh, row0, pos0, n_tok, c_off, n_col, page0, n_pages, slot, k, _ = (int(x) for x in u[:12])
+        assert 0 < n_col <= cols and n_pages > 0 and (k > 1) == (slot != NO_SLOT) and n_tok == (c_off + n_col - 1) // group + 1
+        assert all(table[seq, p * 16 // bt] >= 0 for p in (page0, page0 + n_pages - 1))
+        for col in range(c_off, c_off + n_col):
+            t, h = row0 + col // group, kvh * group + col % group
+            assert rows[t][0] == seq and rows[t][1] == pos0 + col // group
+            pages.setdefault((t, h), []).append((page0, page0 + n_pages))
+            if k:
+                assert slot + (col // group) * k < c.slots
+                slots.setdefault((t, h), []).append(slot + (col // group) * k)
     for it in items:
         row, kvh, h0, p0, p1, slot, seq, blk0 = (int(x) for x in it)
         assert seq == rows[row][0] and blk0 == table[seq, p0 // 16 * 16 // bt] >= 0
@@ -145,11 +160,11 @@ def test_every_row_walks_what_it_sees(kv, geo, kind):
             r = RowRanges() if kind == "causal" else make_ranges(kind, segs, b)
             lo, hi = (None if x is None else list(x) for x in (r.lo, r.hi))
             for window, n_cu, per_cu, whole in ((0, 256, 8, 0), (333, 80, 4, 0), (0, 12, 16, 1)):
-                rc, waves, items, merges, c = scored_plan(kv, geo, bt, table, segs, lo, hi, window, n_cu, per_cu, whole)
+                rc, waves, items, prompts, merges, c = scored_plan(kv, geo, bt, table, segs, lo, hi, window, n_cu, per_cu, whole)
                 assert rc == N.OK
                 tiles = bt >= 16 and not (kv == "q8_0" and geo[2] == 96) and geo[2] <= 256
-                assert (len(waves) > 0) == tiles and (len(items) > 0) != tiles
-                check(kv, geo, bt, table, segs, lo, hi, window, waves, items, merges, c)
+                assert (len(waves) + len(prompts) > 0) == tiles and (len(items) > 0) != tiles
+                check(kv, geo, bt, table, segs, lo, hi, window, waves, items, prompts, merges, c)
 
 
 def test_units_walk_their_documents_only():
@@ -157,13 +172,13 @@ def test_units_walk_their_documents_only():
     n = 48
     segs = [(i, i, 1, 8000) for i in range(n)]
     table = contiguous_table([8001] * n, 16)
-    rc, waves, _, _, _ = scored_plan("bf16", (40, 8, 128, 128), 16, table, segs, [7900] * n, None)
+    rc, waves, _, _, _, _ = scored_plan("bf16", (40, 8, 128, 128), 16, table, segs, [7900] * n, None)
     assert rc == N.OK and int(waves[:, 4].sum()) == n * 8 * (8000 // 16 - 7900 // 16 + 1)
     r = RowRanges.of([(0, 0, 8192, 0)], documents=[list(range(0, 8192, 512))])
     table = contiguous_table([8192], 16)
-    rc, waves, _, _, c = scored_plan("f16", (16, 4, 64, 64), 16, table, [(0, 0, 8192, 0)], list(r.lo), list(r.hi))
-    causal = sum((t // 512 * 0 + t % 512) // 16 + 1 for t in range(0, 8192, 8))   # 32 columns of a group of 4: 8 rows a unit
-    assert rc == N.OK and int(waves[:, 4].sum()) <= 4 * (causal + 1024)
+    rc, waves, _, prompts, _, c = scored_plan("f16", (16, 4, 64, 64), 16, table, [(0, 0, 8192, 0)], list(r.lo), list(r.hi))
+    assert rc == N.OK and len(waves) == 0 and len(prompts) == 4 * 8192 // 64   # 256 columns of a group of 4: 64 rows a unit
+    assert int(prompts[:, 8].sum()) == 4 * 16 * sum(4 * (i + 1) for i in range(8))
 
 
 def test_refused_ranges():
