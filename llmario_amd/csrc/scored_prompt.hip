@@ -55,7 +55,7 @@ __device__ inline float page_value(const uint8_t* head, uint32_t sub, uint32_t t
 // Column (row, head) of a unit in f32 from the pages, one wave: lanes over keys for the scores, over dims for the sums.
 // out: the row's HD values, or its partial (raw sums, then reference and sum).
 template <int KVT, int HD>
-__device__ __noinline__ void redo(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, uint32_t seq, uint32_t kvh, uint32_t head,
+__device__ __forceinline__ void redo(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, uint32_t seq, uint32_t kvh, uint32_t head,
                                   uint32_t pos, uint32_t first, uint32_t end, const float* q, float* out, bool partial) {
   constexpr int ND = HD / 64;
   const uint32_t lane = threadIdx.x & 63u, bt_mask = (1u << g.bt_shift) - 1u;
@@ -63,11 +63,13 @@ __device__ __noinline__ void redo(const PageGeom& g, const UnitGeom& u, const Sc
   float m = -INFINITY, l = 0.f, o[ND];
   for (int i = 0; i < ND; i++) o[i] = 0.f;
   const float slope = sc.slopes ? sc.slopes[head] * LOG2E : 0.f;
+#pragma clang loop unroll(disable)
   for (uint32_t k0 = first; k0 < end; k0 += 64) {
     const uint32_t key = min(k0 + lane, end - 1), n = min(64u, end - k0);
     const uint8_t* b = g.pool + (size_t)(uint32_t)tab[key >> g.bt_shift] * g.block_bytes;
     const uint8_t* kh = b + g.k_off + (size_t)kvh * g.k_head;
     float s = 0.f;
+#pragma clang loop unroll(disable)
     for (uint32_t d = 0; d < (uint32_t)HD; d++)
       s = fmaf(q[d], page_value<KVT>(kh, (key & bt_mask) >> 4, g.k_tile, g.k_scale, g.k_tile_s, false, key & 15u, d, HD), s);
     float p[1] = {s * u.scale_log2};
@@ -82,6 +84,7 @@ __device__ __noinline__ void redo(const PageGeom& g, const UnitGeom& u, const Sc
     l = l * alpha + sum;
     m = mn;
     for (int i = 0; i < ND; i++) o[i] *= alpha;
+#pragma clang loop unroll(disable)
     for (uint32_t j = 0; j < n; j++) {
       const uint32_t kj = k0 + j;
       const float wj = __shfl(w, (int)j);
@@ -98,7 +101,9 @@ __device__ __noinline__ void redo(const PageGeom& g, const UnitGeom& u, const Sc
   }
 }
 
-template <int KVT, int HD>
+// CAP, BIAS: the launch has a cap, slopes (a test in the walk would split its code, and the compiler computes a short
+// branch's values ahead of the test).
+template <int KVT, int HD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillItem* items, const float* q, float* out, MergeCopy mc) {
   using C = Shape<KVT, HD>;
@@ -169,11 +174,11 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
   ids(1);
 
   // ---- Q of the wave's columns (the B operand of S^T = K Q^T), while the first tile is on its way
-  uint32_t ct[NCB], ch[NCB], clo[NCB], cend[NCB], cpos[NCB];
+  uint32_t ct[NCB], ch[NCB], clo[NCB], clen[NCB], cpos[NCB];   // a column sees keys clo .. clo + clen - 1 of the unit's
   bool cv[NCB];
   float slope[NCB], qscale[NCB];
   uint32_t lo_max = 0, end_min = ~0u, lo_min = ~0u, end_max = 0;
-  bool any = false;
+  bool any = false;   // some column of the wave sees a key
 #pragma unroll
   for (int x = 0; x < NCB; x++) {
     const uint32_t c = w * COLS + 16 * x + hq;
@@ -182,19 +187,21 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
     ch[x] = cv[x] ? (c + c_off) - ct[x] * G : 0;
     cpos[x] = pos0 + ct[x];
     clo[x] = (u.window > 0 && cpos[x] + 1 > u.window) ? cpos[x] + 1 - u.window : 0;
-    cend[x] = cpos[x];
+    uint32_t last = cpos[x];
     if (sc.ranges) {
       const uint2 r = sc.ranges[row0 + ct[x]];
       clo[x] = r.x;
-      cend[x] = r.y;
+      last = r.y;
     }
-    slope[x] = sc.slopes && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
+    last = min(last, (page_end << 4) - 1);
+    clen[x] = clo[x] <= last ? last + 1 - clo[x] : 0;
+    slope[x] = BIAS && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
     if (cv[x]) {
       lo_max = max(lo_max, clo[x]);
-      end_min = min(end_min, cend[x]);
-      if (clo[x] <= cend[x]) {
+      end_min = min(end_min, last);
+      if (clen[x]) {
         lo_min = min(lo_min, clo[x]);
-        end_max = max(end_max, cend[x]);
+        end_max = max(end_max, last);
         any = true;
       }
     }
@@ -302,8 +309,13 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
   typedef float f2 __attribute__((ext_vector_type(2)));
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   u16x2 k_top = 0;   // largest |K| bits written by this lane (bf16, q8_0): 0x7c00 and more left f16's range
+  const bool plain = k_mul == 1.f && v_mul == 1.f;   // uniform
   auto widen = [&](uint32_t x, float mul) -> uint32_t {   // two bf16
-    const f2 y = f2{__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)} * mul;
+    f2 y = f2{__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)};
+    if (!plain) {
+      y *= mul;
+      asm volatile("" : "+v"(y));   // not ahead of the test
+    }
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(y, h2));
   };
   auto widen4 = [&](uint4 x, float mul) -> uint4 { return make_uint4(widen(x.x, mul), widen(x.y, mul), widen(x.z, mul), widen(x.w, mul)); };
@@ -380,12 +392,15 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
   __syncthreads();
 
   // ---- the walk
-  constexpr float UP = 7.0f;   // weights are taken against m - 7 (up to 2^15 with the lazy reference): more of them in f16's range
-  float m[NCB], lsum[NCB];
+  constexpr float UP = 7.0f;   // weights up to 2^15: more of them in f16's range
+  // a column's weights are taken against mref = m - UP, m a score of it that none exceeds by more than 8 (room: how far
+  // scores may exceed mref; -inf before its first, while every score is -inf)
+  float mref[NCB], room[NCB], lsum[NCB];
   f4 O[NCB][NJ];
 #pragma unroll
   for (int x = 0; x < NCB; x++) {
-    m[x] = -INFINITY;
+    mref[x] = 0.f;
+    room[x] = -INFINITY;
     lsum[x] = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; j++) O[x][j] = f4{0.f, 0.f, 0.f, 0.f};
@@ -400,7 +415,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const uint32_t key0 = ((page0 + 4 * t) << 4) + 32 * h;
-      if (!any || key0 > end_max || key0 + 31 < lo_min || key0 >= page_end << 4) continue;   // uniform over the wave
+      if (!any || key0 > end_max || key0 + 31 < lo_min) continue;   // uniform over the wave
       f4 s[NCB][2];
 #pragma unroll
       for (int x = 0; x < NCB; x++) s[x][0] = s[x][1] = f4{0.f, 0.f, 0.f, 0.f};
@@ -420,37 +435,55 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
             for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qp[0][x][c], s[x][kk], 0, 0, 0);
           }
         }
-      const bool need_mask = key0 + 31 > end_min || key0 < lo_max || key0 + 32 > page_end << 4;
+      // the first of V's operands on their way before the softmax
+      constexpr int VP = 4;
+      const uint8_t* const vst = st + C::PARTS * C::SIDE + h * NJ * 1024;
+      h8 vpre[VP];
+#pragma unroll
+      for (int j = 0; j < VP; j++) vpre[j] = *(const h8*)(vst + j * 1024);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool need_mask = key0 + 31 > end_min || key0 < lo_max;
       h8 ph[NCB], pl[NCB];
 #pragma unroll
       for (int x = 0; x < NCB; x++) {
-        float p[8];
+        float p[8];   // scores less the reference mref
+        if constexpr (CAP) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = s[x][i >> 2][i & 3] * qscale[x];
-        if (sc.cap_log2 > 0.f) cap_scores<8>(p, sc.cap_log2);
-        if (sc.slopes) bias_scores<8>(p, slope[x], (float)(int)(key0 + 4 * grp - cpos[x]), [](int i) { return (float)(16 * (i >> 2) + (i & 3)); });
+          for (int i = 0; i < 8; i++) p[i] = s[x][i >> 2][i & 3] * qscale[x];
+          cap_scores<8>(p, sc.cap_log2);
+#pragma unroll
+          for (int i = 0; i < 8; i++) p[i] -= mref[x];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) p[i] = fmaf(s[x][i >> 2][i & 3], qscale[x], -mref[x]);
+        }
+        if constexpr (BIAS) bias_scores<8>(p, slope[x], (float)(int)(key0 + 4 * grp - cpos[x]), [](int i) { return (float)(16 * (i >> 2) + (i & 3)); });
         if (need_mask) {
+          const uint32_t at = key0 + 4 * grp - clo[x];   // (keys before clo wrap round)
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            const uint32_t key = key0 + 16 * (i >> 2) + 4 * grp + (i & 3);
-            if (key > cend[x] || key < clo[x] || key >= page_end << 4) p[i] = -INFINITY;
+            p[i] = at + 16 * (i >> 2) + (i & 3) < clen[x] ? p[i] : -INFINITY;
+            asm volatile("" : "+v"(p[i]));   // not ahead of the test
           }
         }
         float lm = p[0];
 #pragma unroll
         for (int i = 1; i < 8; i++) lm = fmaxf(lm, p[i]);
-        if (__ballot(lm > m[x] + 8.0f)) {
-          const float tm = xmax_groups(lm);
-          const float mn = tm > m[x] + 8.0f ? tm : m[x];
-          const float alpha = mn == m[x] ? 1.f : (m[x] == -INFINITY ? 0.f : exp2_fast(m[x] - mn));
-          lsum[x] *= alpha;
+        if (__ballot(lm > room[x])) {   // some column's largest score is 8 past its m, or its first
+          const float tm = xmax_groups(lm) + mref[x];
+          if (tm - mref[x] > room[x]) {
+            const float nref = tm - UP, alpha = room[x] == -INFINITY ? 0.f : exp2_fast(mref[x] - nref);
+            lsum[x] *= alpha;
 #pragma unroll
-          for (int j = 0; j < NJ; j++) O[x][j] *= alpha;
-          m[x] = mn;
+            for (int j = 0; j < NJ; j++) O[x][j] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[i] -= nref - mref[x];
+            mref[x] = nref;
+            room[x] = UP + 8.0f;
+          }
         }
-        const float mref = m[x] == -INFINITY ? 0.f : m[x] - UP;   // every score is -inf while m is
 #pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = exp2_fast(p[i] - mref);
+        for (int i = 0; i < 8; i++) p[i] = exp2_fast(p[i]);
         lsum[x] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         uint32_t hw[4], lw[4];
 #pragma unroll
@@ -460,8 +493,8 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
       }
 #pragma unroll
       for (int j = 0; j < NJ; j++) {
-        const uint8_t* at = st + C::PARTS * C::SIDE + (h * NJ + j) * 1024;
-        const h8 va = *(const h8*)at;
+        const uint8_t* at = vst + j * 1024;
+        const h8 va = j < VP ? vpre[j < VP ? j : 0] : *(const h8*)at;
 #pragma unroll
         for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[x], O[x][j], 0, 0, 0);
 #pragma unroll
@@ -496,6 +529,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
     return u.part + ((size_t)(slot + tok * stride) * u.ng + head) * (HD + 4);
   };
   if (__builtin_expect(__ballot(bad) != 0, 0)) {
+#pragma clang loop unroll(disable)
     for (uint32_t c = 0; c < (uint32_t)COLS && w * COLS + c < n_col; c++) {
       const uint32_t a = w * COLS + c + c_off, tok = a / G, head = a - tok * G, pos = pos0 + tok;
       uint32_t first = (u.window > 0 && pos + 1 > u.window) ? pos + 1 - u.window : 0, last = pos;
@@ -523,7 +557,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
       *(f4u*)(op + 16 * j + 4 * grp) = f4u{o[0], o[1], o[2], o[3]};
     }
     if (slot != NO_SLOT && grp == 0) {
-      op[HD] = m[x] - UP;   // the reference the weights were taken against
+      op[HD] = room[x] == -INFINITY ? -INFINITY : mref[x];   // the reference the weights were taken against
       op[HD + 1] = lsum[x];
     }
   }
@@ -558,7 +592,16 @@ hipError_t launch_scored_prompts(const PageGeom& g, const UnitGeom& u, const Sco
   hipError_t e = hipErrorInvalidValue;
   with_prompt(g.kv_type, g.hd, g.hdv, g.layout, [&](auto t, auto h) {
     constexpr int T = decltype(t)::value, H = decltype(h)::value;
-    LMH_LAUNCH(ev, (scored_prompt_kernel<T, H>), dim3(n_items), dim3(NTH), (Shape<T, H>::LDS), s, g, u, sc, items, q, out, mc);
+#define LMH_PROMPT(CAP, BIAS) \
+  LMH_LAUNCH(ev, (scored_prompt_kernel<T, H, CAP, BIAS>), dim3(n_items), dim3(NTH), (Shape<T, H>::LDS), s, g, u, sc, items, q, out, mc)
+    if (sc.cap_log2 > 0.f) {
+      if (sc.slopes) LMH_PROMPT(true, true);
+      else LMH_PROMPT(true, false);
+    } else {
+      if (sc.slopes) LMH_PROMPT(false, true);
+      else LMH_PROMPT(false, false);
+    }
+#undef LMH_PROMPT
     e = hipGetLastError();
   });
   return e;
