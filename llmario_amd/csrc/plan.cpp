@@ -463,11 +463,18 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
   return true;
 }
 
-// Segments of at least this many columns (rows x query heads of a KV head) run on the kernel for long segments.
+// Segments of at least this many columns (rows x query heads of a KV head) run on the kernel for long segments. 8
+// sequences on 2,000 keys, 32/8 heads of 128, bf16, us: 4 rows each 33.1 so, 27.0 in the unit launch; 16 36.6 and 38.0; 32
+// 42.9 and 43.7; q8_0 32 rows 49.0 and 50.9, 16 42.2 and 41.2; 32 sequences of 16 rows 86.5 and 85.0, q8_0 108 and 87; one
+// prompt of 2,048 a fourth of the unit launch's time less a third.
 constexpr uint64_t PROMPT_MIN_COLS = 128;
-// A unit's fixed cost (its Q, the first tile's way through LDS, its stores) and that of a merge launch, in 64-key tiles.
-constexpr uint64_t PROMPT_UNIT_COST = 4, PROMPT_MERGE_COST = 4;
-constexpr uint64_t PROMPT_MIN_PIECE = 8;   // tiles of a key piece
+// A unit's fixed cost (its Q, the first tile's way through LDS, its stores) and that of a merge launch, in 64-key tiles
+// (~3.5 us of a workgroup at 256 columns; half that on heads of 64). Two prompts of 700 rows, us, whole / in pieces: q8_0
+// 62.6 / 57.9, 256-wide 57.1 / 54.0, with a window and decode rows 85.7 / 71.1, 64-wide 20.8 / 26.7.
+constexpr uint64_t PROMPT_UNIT_COST = 4;
+uint64_t prompt_merge_cost(uint32_t hd) { return hd <= 64 ? 4 : 2; }
+// Tiles of a key piece at the least (2 x 64 rows on 2,000 keys, bf16: 48.6 us at 8, 41.2 at 4, 38.3 at 2 and at 1).
+constexpr uint64_t PROMPT_MIN_PIECE = 2;
 
 // Shaped scores: the units of the segments listed, a workgroup each, the longest first (the device takes them in order, so
 // the last to finish are short). A KV head's units are n_kv apart, so with 8 KV heads (or 4, or 2) those that read the same
@@ -502,7 +509,7 @@ void plan_prompts(const PlanIn& in, const std::vector<uint32_t>& segs, PlanOut& 
   total *= in.n_kv;
   // whole units finish no sooner than the longest, or than an even share; pieces of `even` tiles with the merge
   const uint64_t even = std::max<uint64_t>(PROMPT_MIN_PIECE, (total + in.n_cu - 1) / in.n_cu);
-  const bool cut = !in.prefill_no_split && in.hdv <= 256 && longest > even + even / 4 + PROMPT_MERGE_COST;
+  const bool cut = !in.prefill_no_split && in.hdv <= 256 && longest > even + even / 4 + prompt_merge_cost(in.hd);
   struct Piece {
     uint32_t block, tile0, tiles, k, at;
   };
@@ -607,6 +614,30 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
       else if (in.segs[i].n > 0) rest.push_back(in.segs[i]);
     }
     if (!longer.empty()) {
+      // Few short segments go along, a workgroup each, rather than in a launch of their own (~10 us and its share of the
+      // merge): while they take the device less than that, or than an eighth of the long ones' time. (4 decode rows beside two prompts of ~850 rows,
+      // window 1,024, 16/4 heads of 256: 71 us in two launches, 62 in one.)
+      auto tiles_of = [&](const lmh_seg& sg) -> uint64_t {
+        uint64_t n = 0;
+        const uint64_t cols = sg.n * group;
+        for (uint64_t c0 = 0; c0 < cols; c0 += in.prompt_cols) {
+          const auto p = pages_seen(in, sg, c0 / group, (std::min<uint64_t>(cols, c0 + in.prompt_cols) - 1) / group);
+          n += (p.second - p.first + 4) / 4 + PROMPT_UNIT_COST;
+        }
+        return n;
+      };
+      uint64_t of_long = 0, of_rest = 0;
+      for (uint32_t i : longer) of_long += tiles_of(in.segs[i]);
+      for (const lmh_seg& sg : rest) of_rest += tiles_of(sg);
+      if (8 * of_rest <= of_long || of_rest * in.n_kv <= 3ull * in.n_cu) {
+        longer.clear();
+        for (uint64_t i = 0; i < in.n_segs; i++)
+          if (in.segs[i].n > 0) longer.push_back((uint32_t)i);
+        rest.clear();
+      } else if (of_long * in.n_kv <= 3ull * in.n_cu) {   // and the other way round
+        plan_units(in, o);
+        return;
+      }
       plan_prompts(in, longer, o);
       if (rest.empty()) return;
       PlanIn less = in;

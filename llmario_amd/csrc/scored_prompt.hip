@@ -1,8 +1,10 @@
 // scored_prompt.hip — attention with shaped scores (lmh_attend_scored) of long segments on gfx950 matrix cores.
 //
 // A unit is up to 8 * COLS columns (token, query head) of one segment and KV head, flattened token-major as
-// units.hip's, over the key pages its columns see; one workgroup of 8 waves (two per SIMD) takes a unit, wave w its
-// columns COLS * w .. (COLS: 32 as two 16-column blocks; 16 on 256-wide heads). The workgroup walks 64-key tiles:
+// units.hip's, over the key pages its columns see; one workgroup of 8 waves (two per SIMD, four on heads of 64) takes a unit, wave w its
+// columns COLS * w .. (COLS: 32 as two 16-column blocks on heads of 128; 16 on 256, whose O and Q fill the registers of
+// two waves per SIMD, and on 64, where two workgroups to a CU hide each other's latencies: 8,192 packed tokens of 16
+// heads 46 us against 56 with 32 columns). The workgroup walks 64-key tiles:
 // all its waves share each tile's K and V through LDS, so pages are read once per unit and expanded once:
 //   f16: as they are. bf16: widened to f16. q8_0: code * scale as f16 hi + lo parts (exact: 7 + 11 bits).
 //   S^T[keys x cols] = K . Q^T       v_mfma_f32_16x16x32_f16, Q as f16 hi + lo parts of the column scaled by a
@@ -28,7 +30,7 @@ constexpr int PW = 8, NTH = 64 * PW, BK = 64;
 template <int KVT, int HD>
 struct Shape {
   static constexpr bool Q8 = KVT == KV_Q8, BF = KVT == KV_BF16;
-  static constexpr int NCB = HD <= 128 ? 2 : 1, COLS = 16 * NCB;
+  static constexpr int NCB = HD == 128 ? 2 : 1, COLS = 16 * NCB;
   static constexpr int NC = HD / 32, NJ = HD / 16;
   static constexpr int SIDE = BK * HD * 2;                  // bytes of a tile's K or V part in LDS
   static constexpr int PARTS = Q8 ? 2 : 1;
@@ -104,7 +106,7 @@ __device__ __forceinline__ void redo(const PageGeom& g, const UnitGeom& u, const
 // CAP, BIAS: the launch has a cap, slopes (a test in the walk would split its code, and the compiler computes a short
 // branch's values ahead of the test).
 template <int KVT, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : 2, HD == 64 ? 4 : 2)))
 void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillItem* items, const float* q, float* out, MergeCopy mc) {
   using C = Shape<KVT, HD>;
   constexpr bool Q8 = C::Q8, BF = C::BF;
@@ -145,7 +147,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
 #pragma unroll
     for (int i = 0; i < NI; i++)
 #pragma unroll
-      for (int r = 0; r < C::ROWS_I; r++) blk[i][r] = tab[(page_of(t, i, r) << 4) >> g.bt_shift];
+      for (int r = 0; r < C::ROWS_I; r++) blk[i][r] = r == 1 && NI > 1 && is_k(i) ? blk[i][0] : tab[(page_of(t, i, r) << 4) >> g.bt_shift];
   };
   uint4 raw[NI][C::ROWS_I];
   uint32_t rs[NI][Q8 ? 4 : 1];   // q8_0: the scales (K: the key's two chunks; V: of four keys)

@@ -82,7 +82,7 @@ def check(kv, geo, bt, table, segs, lo, hi, window, waves, items, prompts, merge
                 assert slot + (col // group) * k < c.slots
                 slots.setdefault((t, h), []).append(slot + (col // group) * k)
         at += n
-    cols = 128 if geo[2] == 256 else 256
+    cols = 256 if geo[2] == 128 else 128
     assert all(int(a[8]) + 3 >= int(b[8]) for a, b in zip(prompts, prompts[1:]))   # the longest first (in 64-key tiles)
     for u in prompts:
         seq, kvh, row0, pos0, n_tok, c_off, n_col, page0, n_pages, slot, k, _ = (int(x) for x in u[:12])
@@ -177,8 +177,8 @@ def test_units_walk_their_documents_only():
     r = RowRanges.of([(0, 0, 8192, 0)], documents=[list(range(0, 8192, 512))])
     table = contiguous_table([8192], 16)
     rc, waves, _, prompts, _, c = scored_plan("f16", (16, 4, 64, 64), 16, table, [(0, 0, 8192, 0)], list(r.lo), list(r.hi))
-    assert rc == N.OK and len(waves) == 0 and len(prompts) == 4 * 8192 // 64   # 256 columns of a group of 4: 64 rows a unit
-    assert int(prompts[:, 8].sum()) == 4 * 16 * sum(4 * (i + 1) for i in range(8))
+    assert rc == N.OK and len(waves) == 0 and len(prompts) == 4 * 8192 // 32   # 128 columns of a group of 4: 32 rows a unit
+    assert int(prompts[:, 8].sum()) == 4 * 16 * sum(2 * (i + 1) for i in range(16))
 
 
 def test_refused_ranges():
