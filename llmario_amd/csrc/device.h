@@ -154,6 +154,9 @@ hipError_t launch_store_encoded(const PageGeom& g, const int32_t* row_seq, const
                                 uint32_t v_row, hipStream_t s);
 hipError_t launch_gather(const PageGeom& g, const int32_t* row_seq, const int32_t* row_pos, uint32_t n_rows,
                          float* k, float* v, hipStream_t s);
+// Runs of up to 16 rows of one page tile (RopeRow: first row, position, block; pad: rows), f16 / bf16 tiles, k and v
+// 16-byte aligned; f32: decoded, else the rows' encoding.
+hipError_t launch_gather_runs(const PageGeom& g, const RopeRow* runs, uint32_t n_runs, bool f32, uint8_t* k, uint8_t* v, hipStream_t s);
 hipError_t launch_gather_encoded(const PageGeom& g, const int32_t* row_seq, const int32_t* row_pos,
                                  uint32_t n_rows, uint8_t* k, uint8_t* v, uint32_t k_row, uint32_t v_row,
                                  hipStream_t s);

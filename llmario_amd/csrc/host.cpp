@@ -243,6 +243,12 @@ struct PageOp {
   int32_t win = 0;  // 1: a block of the window pool (zeroing only)
 };
 
+// What a table of turns (lmh_qk_rope_store_axes) depends on.
+struct RopeTurns {
+  float theta, freq_scale;
+  uint32_t rot_dim, n_axes, flags, sections[4];
+};
+
 }  // namespace
 
 struct lmh_kv {
@@ -286,6 +292,8 @@ struct lmh_kv {
   double acc_ms[6] = {0, 0, 0, 0, 0, 0};
   uint64_t launches[6] = {0, 0, 0, 0, 0, 0};
   std::vector<uint8_t> payload;
+  std::vector<double> turns;                // the latest lmh_qk_rope_store_axes call's, and what they are of
+  RopeTurns turns_of{};
   std::vector<KeyRange> ranges;             // lmh_attend_scored: the keys each row sees
   std::vector<lmh_sched*> scheds;           // schedulers bound to this handle
   // ---- lmh_attend planning / precision options (lmh_kv_set_tuning)
@@ -1326,10 +1334,26 @@ static int32_t kv_io(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n
   const int32_t *rs, *rp;
   const uint8_t* ex;
   int slot;
-  if ((rc = kv->stage_rows(nullptr, 0, nullptr, 0, rs, rp, ex, slot)) != LMH_OK) return rc;
-  const PageGeom g = kv->geom(layer);
   const LayerLayout& y = kv->layers[layer];
+  // reads of 16-bit tiles: in runs of rows that share a page tile
+  std::vector<RopeRow> runs;
+  if (mode >= 2 && y.layout == LAYOUT_TILES && (kv->kv_type == LMH_KV_F16 || kv->kv_type == LMH_KV_BF16) && ((uintptr_t)a | (uintptr_t)b) % 16 == 0) {
+    const std::vector<int32_t>& tab = y.win ? kv->h_wtable : kv->h_table;
+    for (uint64_t i = 0; i < n_segs; i++)
+      for (uint64_t j = 0; j < segs[i].n;) {
+        const uint64_t pos = segs[i].pos0 + j, n = std::min<uint64_t>(16 - pos % 16, segs[i].n - j);
+        runs.push_back(RopeRow{(uint32_t)(segs[i].start + j), (uint32_t)pos, (uint32_t)tab[segs[i].seq * kv->bps + (pos >> kv->bt_shift)], (uint32_t)n});
+        j += n;
+      }
+  }
+  if ((rc = kv->stage_rows(runs.data(), runs.size() * sizeof(RopeRow), nullptr, 0, rs, rp, ex, slot)) != LMH_OK) return rc;
+  const PageGeom g = kv->geom(layer);
   hipError_t e = hipSuccess;
+  if (!runs.empty()) {
+    e = launch_gather_runs(g, (const RopeRow*)ex, (uint32_t)runs.size(), mode == 2, (uint8_t*)a, (uint8_t*)b, st);
+    if (e != hipSuccess) return kv->hip_fail(e, "kernel launch");
+    return kv->release_rows(slot, st);
+  }
   switch (mode) {
     case 0: e = launch_store_f32(g, rs, rp, (uint32_t)n_rows, (const float*)a, (const float*)b, st); break;
     case 1:
@@ -1436,10 +1460,14 @@ static int32_t rope_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64
   const uint32_t half_rot = apply ? p->rot_dim / 2 : 0;
   // (axes: 64-bit turns in its place)
   std::vector<float> freq(std::max<uint32_t>(axes ? 2 * half_rot : half_rot, 1), 0.f);
-  std::vector<double> turns(axes ? half_rot : 0);
-  if (axes) {
-    axes_turns(axes, p, turns.data());
-    std::memcpy(freq.data(), turns.data(), half_rot * sizeof(double));
+  if (axes) {   // 64 powers take ~3 us: kept for the next call of the same rotation
+    const RopeTurns of{p->theta, p->freq_scale, p->rot_dim, axes->n_axes, axes->flags, {axes->sections[0], axes->sections[1], axes->sections[2], axes->sections[3]}};
+    if (kv->turns.size() != half_rot || std::memcmp(&of, &kv->turns_of, sizeof of) != 0) {
+      kv->turns.resize(half_rot);
+      axes_turns(axes, p, kv->turns.data());
+      kv->turns_of = of;
+    }
+    std::memcpy(freq.data(), kv->turns.data(), half_rot * sizeof(double));
   }
   for (uint32_t i = 0; !axes && i < half_rot; i++) freq[i] = powf(p->theta, -(2.0f * (float)i) / (float)p->rot_dim);
   hipStream_t st = (hipStream_t)stream;

@@ -557,6 +557,70 @@ __device__ void gather_enc_side(const PageGeom& g, const Slot& sl, bool is_v, ui
   }
 }
 
+// The rows of a run (up to 16 consecutive positions of one page tile) read back from f16 / bf16 tiles, a wave per (head,
+// side) in turn: the tile is loaded as it lies, 1 KiB a request; a K lane holds 8 dims of a key, which is 16 bytes of that
+// key's row; V (four keys to a lane) is turned in LDS. F32: decoded, else the pages' bits. Row by row, with two-byte reads
+// of lines that eight rows share and one-byte stores, 8,192 rows of 8 heads of 128 took 41 us; so 15.
+template <bool F32>
+__global__ __launch_bounds__(256) void gather_runs_kernel(PageGeom g, const RopeRow* runs, uint8_t* k, uint8_t* v) {
+  __shared__ __attribute__((aligned(16))) uint8_t turn[4][8][1040];   // rows of 1 KiB, 16 bytes apart: other banks
+  const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
+  const RopeRow rr = runs[blockIdx.x];
+  const uint32_t n = rr.pad, m0 = rr.pos & 15u, sub = (rr.pos & ((1u << g.bt_shift) - 1u)) >> 4;
+  const uint8_t* b = g.pool + (size_t)rr.blk * g.block_bytes;
+  const bool f16 = g.kv_type == KV_F16;
+  auto put = [&](uint8_t* dst, size_t at, uint4 x) {   // eight values at element `at` of a side's rows
+    if constexpr (F32) {
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const uint16_t h = (uint16_t)(i & 1 ? u[i >> 1] >> 16 : u[i >> 1]);
+        f[i] = f16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+      }
+      float4* o = (float4*)((float*)dst + at);
+      o[0] = make_float4(f[0], f[1], f[2], f[3]);
+      o[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      *(uint4*)(dst + 2 * at) = x;
+    }
+  };
+  for (uint32_t it = blockIdx.y * 4 + w; it < 2 * g.n_kv; it += gridDim.y * 4) {   // a wave's own: no barrier below
+    const bool is_v = it >= g.n_kv;
+    const uint32_t h = is_v ? it - g.n_kv : it, dim = is_v ? g.hdv : g.hd;
+    const uint8_t* t = b + (is_v ? g.v_off + (size_t)h * g.v_head + (size_t)sub * g.v_tile : g.k_off + (size_t)h * g.k_head + (size_t)sub * g.k_tile);
+    uint4 x[8];
+#pragma unroll
+    for (uint32_t c = 0; c < 8; c++)
+      if (c < dim / 32) x[c] = *(const uint4*)(t + c * 1024 + lane * 16);
+    if (!is_v) {
+      const uint32_t m = lane & 15u;
+      if (m < m0 || m >= m0 + n) continue;
+#pragma unroll
+      for (uint32_t c = 0; c < 8; c++)
+        if (c < dim / 32) put(k, ((size_t)(rr.row + m - m0) * g.n_kv + h) * dim + 32 * c + 8 * (lane >> 4), x[c]);
+      continue;
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < 8; c++)
+      if (c < dim / 32) *(uint4*)&turn[w][c][lane * 16] = x[c];
+    wave_lds_sync();
+    for (uint32_t i = lane; i < 2 * dim; i += 64) {   // piece i: key i / (dim / 8), dims 8 (i % (dim / 8)) ..
+      const uint32_t m = i / (dim / 8), d = i % (dim / 8) * 8;
+      if (m < m0 || m >= m0 + n) continue;
+      uint32_t u[4];
+#pragma unroll
+      for (uint32_t e = 0; e < 4; e++) {
+        const uint32_t o = v16_off(m, d + 2 * e) & 1023u;   // the next dim: 16 bytes on
+        const uint8_t* p = &turn[w][d >> 5][o];
+        u[e] = *(const uint16_t*)p | (uint32_t)*(const uint16_t*)(p + 16) << 16;
+      }
+      put(v, ((size_t)(rr.row + m - m0) * g.n_kv + h) * dim + d, make_uint4(u[0], u[1], u[2], u[3]));
+    }
+    wave_lds_sync();
+  }
+}
+
 __global__ void gather_encoded_kernel(PageGeom g, const int32_t* row_seq, const int32_t* row_pos, uint8_t* k,
                                       uint8_t* v, uint32_t k_row, uint32_t v_row) {
   const uint32_t row = blockIdx.x;
@@ -1467,6 +1531,17 @@ hipError_t launch_gather(const PageGeom& g, const int32_t* row_seq, const int32_
   return hipGetLastError();
 }
 
+hipError_t launch_gather_runs(const PageGeom& g, const RopeRow* runs, uint32_t n_runs, bool f32, uint8_t* k, uint8_t* v, hipStream_t s) {
+  if (n_runs == 0) return hipSuccess;
+  if (g.layout != LAYOUT_TILES || (g.kv_type != KV_F16 && g.kv_type != KV_BF16) || g.hd % 32 || g.hdv % 32 || g.hd > 256 || g.hdv > 256)
+    return hipErrorInvalidValue;
+  // a wave's share: every (head, side) of a run in long calls, down to one where runs are few
+  const uint32_t most = (2 * g.n_kv + 3) / 4, split = std::min(most, std::max(1u, 2048u / n_runs));
+  const dim3 grid(n_runs, split);
+  if (f32) hipLaunchKernelGGL((gather_runs_kernel<true>), grid, dim3(256), 0, s, g, runs, k, v);
+  else hipLaunchKernelGGL((gather_runs_kernel<false>), grid, dim3(256), 0, s, g, runs, k, v);
+  return hipGetLastError();
+}
 hipError_t launch_gather_encoded(const PageGeom& g, const int32_t* row_seq, const int32_t* row_pos,
                                  uint32_t n_rows, uint8_t* k, uint8_t* v, uint32_t k_row, uint32_t v_row,
                                  hipStream_t s) {

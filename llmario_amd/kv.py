@@ -57,6 +57,11 @@ class Segments:
         self.segs = [tuple(int(x) for x in s) for s in segs]
         self.arr = (N.Seg * max(len(self.segs), 1))(*[N.Seg(*s) for s in self.segs])
         self.n = len(self.segs)
+        self.rows = sum(s[2] for s in self.segs)
+
+
+def _rows(segs):
+    return segs.rows if isinstance(segs, Segments) else sum(int(s[2]) for s in segs)
 
 
 def _segs(segs):
@@ -320,7 +325,7 @@ class HipKvCache:
         sections = [int(x) for x in sections]
         if not 1 <= len(sections) <= 4 or min(sections) < 0:
             raise ValueError("sections: the pairs of 1 to 4 axes")
-        n_rows = sum(int(s.n) for s in arr[:n])
+        n_rows = _rows(segs)
         if positions.dtype != torch.int32 or not positions.is_cuda or not positions.is_contiguous() or \
                 tuple(positions.shape) != (len(sections), n_rows):
             raise ValueError("positions must be a contiguous int32 cuda tensor [n_axes, n_rows]")
@@ -360,8 +365,8 @@ class HipKvCache:
         slopes[head] * |position - key| (slopes: [n_head] f32 cuda tensor or None), and whose rows see the keys that
         `ranges` (RowRanges, or None: causal) and `window` leave them; a row that sees none is zeros."""
         arr, n = _segs(segs)
-        if ranges is not None and ranges.n is not None and ranges.n != sum(int(s.n) for s in arr[:n]):
-            raise ValueError(f"ranges of {ranges.n} rows for a batch of {sum(int(s.n) for s in arr[:n])}")
+        if ranges is not None and ranges.n is not None and ranges.n != _rows(segs):
+            raise ValueError(f"ranges of {ranges.n} rows for a batch of {_rows(segs)}")
         if slopes is not None and 0 <= layer < len(self.layers):   # the library checks the layer
             import torch
             if slopes.dtype != torch.float32 or not slopes.is_cuda or not slopes.is_contiguous() or slopes.numel() != self.layers[layer].n_head:
