@@ -433,8 +433,8 @@ int32_t lmh_plan_unit_waves(const lmh_plan_desc* d, const lmh_seg* segs, uint64_
                             uint32_t* waves, uint64_t waves_cap, uint32_t* merges, uint64_t merges_cap,
                             lmh_plan_wave_counts* counts);
 /* The same for lmh_attend_scored, whose rows see keys row_lo[t] .. row_hi[t] - 1 (either NULL, as there): the wave
- * records of its unit launch, the units of its long segments (lmh_plan_attend's unit records), or the decode items of
- * a geometry without either, eight words each, and the merges. */
+ * records of its unit launch, the units of its long segments, ten words each, or the decode items of a geometry
+ * without either, eight words each, and the merges. */
 int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_segs, const uint32_t* row_lo,
                         const uint32_t* row_hi, uint32_t waves_per_cu, uint32_t* waves, uint64_t waves_cap,
                         uint32_t* items, uint64_t items_cap, uint32_t* prompts, uint64_t prompts_cap,

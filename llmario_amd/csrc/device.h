@@ -239,7 +239,7 @@ hipError_t launch_scored_rows(const PageGeom& g, const RowGeom& r, const ScoreGe
 // Long segments with shaped scores (scored_prompt.hip): a workgroup per unit of up to scored_prompt_cols columns (0: no
 // instance takes the geometry).
 uint32_t scored_prompt_cols(uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_t layout);
-hipError_t launch_scored_prompts(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, const PrefillItem* items, uint32_t n_items,
+hipError_t launch_scored_prompts(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, const PromptItem* items, uint32_t n_items,
                                  const float* q, float* out, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev = {});
 uint32_t prefill_wg_per_cu();     // prefill workgroups a CU holds when their LDS fits (160 KiB / this)
 uint32_t prefill_cols_per_unit();

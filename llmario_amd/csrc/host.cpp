@@ -617,10 +617,9 @@ struct lmh_kv {
       if (sg.pos0 + sg.n > seqs[sg.seq].blocks.size() * bt)
         return fail(LMH_INVALID_ARGUMENT, "segment positions beyond the sequence's reserved blocks");
       if (sg.pos0 + sg.n > 0x7fffffffull) return fail(LMH_INVALID_ARGUMENT, "position too large");
-      for (uint64_t j = 0; j < sg.n; j++) {
-        row_seq.push_back((int32_t)sg.seq);
-        row_pos.push_back((int32_t)(sg.pos0 + j));
-      }
+      row_seq.resize(n_rows + sg.n, (int32_t)sg.seq);
+      row_pos.resize(n_rows + sg.n);
+      for (uint64_t j = 0; j < sg.n; j++) row_pos[n_rows + j] = (int32_t)(sg.pos0 + j);
       n_rows += sg.n;
     }
     if (n_rows > 0x7fffffffull) return fail(LMH_INVALID_ARGUMENT, "too many rows");
@@ -633,8 +632,8 @@ struct lmh_kv {
   // enqueues every kernel that reads the slot, then calls release_rows(slot, stream).
   int32_t stage_rows(const void* extra, size_t extra_bytes, const void* extra2, size_t extra2_bytes,
                      const int32_t*& d_rs, const int32_t*& d_rp, const uint8_t*& d_extra, int& slot,
-                     bool may_grow = true) {
-    const size_t nr = row_seq.size();
+                     bool may_grow = true, bool with_rows = true) {   // with_rows: some kernel of the call reads the row arrays
+    const size_t nr = with_rows ? row_seq.size() : 0;
     const size_t rows_bytes = (nr * 8 + 255) / 256 * 256;
     const size_t extra_pad = (extra_bytes + 255) / 256 * 256;
     const size_t total = rows_bytes + extra_pad + extra2_bytes;
@@ -1346,7 +1345,7 @@ static int32_t kv_io(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n
         j += n;
       }
   }
-  if ((rc = kv->stage_rows(runs.data(), runs.size() * sizeof(RopeRow), nullptr, 0, rs, rp, ex, slot)) != LMH_OK) return rc;
+  if ((rc = kv->stage_rows(runs.data(), runs.size() * sizeof(RopeRow), nullptr, 0, rs, rp, ex, slot, true, runs.empty())) != LMH_OK) return rc;
   const PageGeom g = kv->geom(layer);
   hipError_t e = hipSuccess;
   if (!runs.empty()) {
@@ -1667,12 +1666,12 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   // one staged payload: [decode items | merges | prefill items], or [merges | ranges | prompts | unit waves], the
   // waves copied to the staging slot straight from the plan
   const size_t uwaves_bytes = kv->plan.uwaves.size() * sizeof(UnitWave);
-  const size_t prompts_bytes = (kv->plan.prompts.size() * sizeof(PrefillItem) + 255) / 256 * 256;
+  const size_t prompts_bytes = (kv->plan.prompts.size() * sizeof(PromptItem) + 255) / 256 * 256;
   const size_t ranges_bytes = ranged && uwaves_bytes + prompts_bytes ? (n_rows * sizeof(KeyRange) + 255) / 256 * 256 : 0;
   kv->payload.resize(items_pad + merges_pad + kv->plan.pitems.size() * sizeof(PrefillItem) + ranges_bytes + prompts_bytes);
   if (ranges_bytes) std::memcpy(kv->payload.data() + items_pad + merges_pad, kv->ranges.data(), n_rows * sizeof(KeyRange));
   if (prompts_bytes)
-    std::memcpy(kv->payload.data() + items_pad + merges_pad + ranges_bytes, kv->plan.prompts.data(), kv->plan.prompts.size() * sizeof(PrefillItem));
+    std::memcpy(kv->payload.data() + items_pad + merges_pad + ranges_bytes, kv->plan.prompts.data(), kv->plan.prompts.size() * sizeof(PromptItem));
   if (items_bytes) std::memcpy(kv->payload.data(), kv->plan.items.data(), items_bytes);
   if (merges_bytes) std::memcpy(kv->payload.data() + items_pad, kv->plan.merges.data(), merges_bytes);
   if (!kv->plan.pitems.empty())
@@ -1702,7 +1701,7 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
     }
   }
   if ((rc = kv->stage_rows(kv->payload.data(), kv->payload.size(), kv->plan.uwaves.data(), uwaves_bytes, rs, rp, ex, slot,
-                           !noalloc)) != LMH_OK)
+                           !noalloc, !sp || items_bytes != 0)) != LMH_OK)
     return rc;
   const PageGeom g = kv->geom(layer);
   RowGeom r{};
@@ -1767,7 +1766,7 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
   const UnitGeom ug{y.n_head, group, r.scale_log2, r.window, ng, pl.u_shared ? 1u : 0u, part};
   if (prompts_bytes) {
     if ((e = time_launch(LMH_KERNEL_PREFILL, ev)) != hipSuccess) return kv->hip_fail(e, "event");
-    e = launch_scored_prompts(g, ug, sg, (const PrefillItem*)(ex + items_pad + merges_pad + ranges_bytes), (uint32_t)pl.prompts.size(),
+    e = launch_scored_prompts(g, ug, sg, (const PromptItem*)(ex + items_pad + merges_pad + ranges_bytes), (uint32_t)pl.prompts.size(),
                               q, out, uwaves_bytes ? MergeCopy{} : mc, st, ev);
     if (e != hipSuccess) return kv->hip_fail(e, "prompt kernel");
   }
@@ -1996,7 +1995,7 @@ int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_
   if (o.uwaves.size() > waves_cap || o.items.size() > items_cap || o.prompts.size() > prompts_cap || o.merges.size() > merges_cap) return LMH_INVALID_ARGUMENT;
   if (!o.uwaves.empty()) std::memcpy(waves, o.uwaves.data(), o.uwaves.size() * sizeof(UnitWave));
   if (!o.items.empty()) std::memcpy(items, o.items.data(), o.items.size() * sizeof(DecodeItem));
-  if (!o.prompts.empty()) std::memcpy(prompts, o.prompts.data(), o.prompts.size() * sizeof(PrefillItem));
+  if (!o.prompts.empty()) std::memcpy(prompts, o.prompts.data(), o.prompts.size() * sizeof(PromptItem));
   if (!o.merges.empty()) std::memcpy(merges, o.merges.data(), o.merges.size() * sizeof(MergeItem));
   return LMH_OK;
 }

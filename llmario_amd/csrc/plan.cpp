@@ -78,14 +78,17 @@ struct WgLists {
 // partial rows (heads x k pieces) one merge wave loads at once: f(token, first head, heads) for each.
 // At most `heads` at a time.
 template <typename F>
-void for_each_merge(const PrefillItem& it, uint64_t group, uint32_t k, F&& f, uint32_t heads = PF_MERGE_ROWS) {
+void for_each_merge(uint32_t n_tok, uint64_t c_off, uint32_t n_col, uint64_t group, uint32_t k, F&& f, uint32_t heads = PF_MERGE_ROWS) {
   const uint32_t hpm = std::max<uint32_t>(1, std::min(heads, PF_MERGE_ROWS / k));
-  const uint64_t c_abs = it.c_off;   // the unit's first column, counted from its first token
-  for (uint32_t i = 0; i < it.n_tok; i++) {
-    const uint64_t h_lo = i == 0 ? c_abs : 0;
-    const uint64_t h_hi = std::min<uint64_t>(group, c_abs + it.n_col - (uint64_t)i * group);
+  for (uint32_t i = 0; i < n_tok; i++) {   // (c_off: the unit's first column, counted from its first token)
+    const uint64_t h_lo = i == 0 ? c_off : 0;
+    const uint64_t h_hi = std::min<uint64_t>(group, c_off + n_col - (uint64_t)i * group);
     for (uint64_t h = h_lo; h < h_hi; h += hpm) f(i, (uint32_t)h, (uint32_t)std::min<uint64_t>(hpm, h_hi - h));
   }
+}
+template <typename F>
+void for_each_merge(const PrefillItem& it, uint64_t group, uint32_t k, F&& f, uint32_t heads = PF_MERGE_ROWS) {
+  for_each_merge(it.n_tok, it.c_off, it.n_col, group, k, f, heads);
 }
 
 // The pages that rows t0 .. t1 of a segment see, first and last (rows that see nothing: the page of the first).
@@ -401,7 +404,8 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
   o.u_nb = nb;
   o.u_w = W;
   auto launch_at = [&](uint32_t wg) { return n_xcd == 1 ? wg : wg % per_xcd * n_xcd + wg / per_xcd; };
-  o.uwaves.assign((size_t)per_xcd * n_xcd * W, UnitWave{});
+  o.uwaves.resize((size_t)per_xcd * n_xcd * W);   // (every record is written below: those of no member idle)
+  std::vector<uint8_t> filled((size_t)per_xcd * n_xcd, 0);   // waves of each workgroup given to members
   // partial slots and merges
   std::vector<uint32_t> slots_of;   // per member: first slot of its unit
   if (cut) {
@@ -426,15 +430,29 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
     const int32_t* tab = in.table + (uint64_t)it.seq * in.bps;
     UnitWave* w = &o.uwaves[(size_t)launch_at(m.wg) * W + m.at];
     const uint32_t n = std::min(m.n, ns);   // (a piece's waves each have a step)
+    const uint32_t per = ns / n, over = ns % n;
+    uint32_t step = 0, carry = 0;   // floor(ns j / n), by increments
     for (uint32_t j = 0; j < n; j++) {
-      const uint32_t a = ns * j / n * KT, b = std::min(n_pages, ns * (j + 1) / n * KT);
+      const uint32_t a = step * KT;
+      step += per;
+      carry += over;
+      if (carry >= n) {
+        carry -= n;
+        step++;
+      }
+      const uint32_t b = std::min(n_pages, step * KT);
       const uint64_t p = page0 + a, p1 = std::min<uint64_t>(p + 1, page0 + b - 1);
       w[j] = UnitWave{it.seq, it.row0, it.pos0, page0 + a, b - a, k ? slots_of[i] + (m.piece & 0xffffu) : NO_SLOT,
                       {(uint32_t)tab[(p << 4) >> in.bt_shift], (uint32_t)tab[(p1 << 4) >> in.bt_shift]},
                       m.kvh | it.c_off << 16, it.n_col | j << 8 | n << 16 | k << 24};
     }
+    for (uint32_t j = n; j < m.n; j++) w[j] = UnitWave{};
+    uint8_t& at = filled[launch_at(m.wg)];
+    at = (uint8_t)std::max<uint32_t>(at, m.at + m.n);
     o.u_shared |= n > 1;
   }
+  for (size_t b = 0; b < filled.size(); b++)
+    for (uint32_t j = filled[b]; j < W; j++) o.uwaves[b * W + j] = UnitWave{};
   o.chunk = c * KT;
   if (in.list_units) {   // as prefill units: pf_wg lists
     std::vector<std::vector<uint32_t>> lists(n_wg);
@@ -482,20 +500,20 @@ constexpr uint64_t PROMPT_MIN_PIECE = 2;
 // one of them, they run as key pieces whose partials a merge combines.
 void plan_prompts(const PlanIn& in, const std::vector<uint32_t>& segs, PlanOut& o) {
   const uint64_t group = in.n_head / in.n_kv;
-  std::vector<PrefillItem> blocks;
+  std::vector<PromptItem> blocks;
+  std::vector<uint32_t> n_tok;   // tokens of each block
   uint64_t total = 0, longest = 0;
   for (uint32_t i : segs) {
     const lmh_seg& sg = in.segs[i];
     const uint64_t n_cols = sg.n * group;
     for (uint64_t c0 = 0; c0 < n_cols; c0 += in.prompt_cols) {
-      PrefillItem it{};
+      PromptItem it{};
       it.n_col = (uint32_t)std::min<uint64_t>(in.prompt_cols, n_cols - c0);
       const uint64_t t0 = c0 / group, t1 = (c0 + it.n_col - 1) / group;
       const auto pages = pages_seen(in, sg, t0, t1);
       it.seq = (uint32_t)sg.seq;
       it.row0 = (uint32_t)(sg.start + t0);
       it.pos0 = (uint32_t)(sg.pos0 + t0);
-      it.n_tok = (uint32_t)(t1 - t0 + 1);
       it.c_off = (uint32_t)(c0 % group);
       it.page0 = (uint32_t)pages.first;
       it.n_pages = (uint32_t)(pages.second - pages.first + 1);
@@ -504,6 +522,7 @@ void plan_prompts(const PlanIn& in, const std::vector<uint32_t>& segs, PlanOut& 
       total += tiles + PROMPT_UNIT_COST;
       longest = std::max(longest, tiles);
       blocks.push_back(it);
+      n_tok.push_back((uint32_t)(t1 - t0 + 1));
     }
   }
   total *= in.n_kv;
@@ -531,25 +550,25 @@ void plan_prompts(const PlanIn& in, const std::vector<uint32_t>& segs, PlanOut& 
   const uint32_t merge_heads = (uint32_t)std::max<uint64_t>(1, cols_cut * in.n_kv / 1024);
   for (const Piece& p : pieces) {
     if (p.k == 1 || p.at != 0) continue;
-    const PrefillItem& it = blocks[p.block];
+    const PromptItem& it = blocks[p.block];
     base[p.block] = o.slots;
     for (uint32_t kvh = 0; kvh < in.n_kv; kvh++) {
       const uint32_t s0 = o.slots;
-      for_each_merge(it, group, p.k, [&](uint32_t t, uint32_t h, uint32_t nh) {
+      for_each_merge(n_tok[p.block], it.c_off, it.n_col, group, p.k, [&](uint32_t t, uint32_t h, uint32_t nh) {
         o.merges.push_back(MergeItem{it.row0 + t, kvh, h, s0 + t * p.k, p.k, nh});
       }, merge_heads);
-      o.slots += it.n_tok * p.k;
+      o.slots += n_tok[p.block] * p.k;
     }
   }
   o.prompts.reserve(pieces.size() * in.n_kv);
   for (const Piece& p : pieces) {
-    PrefillItem it = blocks[p.block];
+    PromptItem it = blocks[p.block];
     it.page0 += 4 * p.tile0;
     it.n_pages = std::min(it.n_pages, 4 * (p.tile0 + p.tiles)) - 4 * p.tile0;
     it.slot_stride = p.k > 1 ? p.k : 0;
     for (uint32_t kvh = 0; kvh < in.n_kv; kvh++) {
       it.kvh = kvh;
-      if (p.k > 1) it.slot = base[p.block] + kvh * it.n_tok * p.k + p.at;
+      if (p.k > 1) it.slot = base[p.block] + kvh * n_tok[p.block] * p.k + p.at;
       o.prompts.push_back(it);
     }
   }
@@ -627,9 +646,11 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
         return n;
       };
       uint64_t of_long = 0, of_rest = 0;
-      for (uint32_t i : longer) of_long += tiles_of(in.segs[i]);
+      if (!rest.empty())
+        for (uint32_t i : longer) of_long += tiles_of(in.segs[i]);
       for (const lmh_seg& sg : rest) of_rest += tiles_of(sg);
-      if (8 * of_rest <= of_long || of_rest * in.n_kv <= 3ull * in.n_cu) {
+      if (rest.empty()) {
+      } else if (8 * of_rest <= of_long || of_rest * in.n_kv <= 3ull * in.n_cu) {
         longer.clear();
         for (uint64_t i = 0; i < in.n_segs; i++)
           if (in.segs[i].n > 0) longer.push_back((uint32_t)i);

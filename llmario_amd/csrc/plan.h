@@ -78,7 +78,7 @@ struct PlanOut {
   std::vector<UnitWave> uwaves;       // a unit launch (units.hip) instead of all of the above but the merges
   uint32_t u_nb = 0, u_w = 0;         // its 16-column blocks per unit and waves per workgroup
   bool u_shared = false;              // some unit is shared between waves
-  std::vector<PrefillItem> prompts;   // scored: units of long segments, a workgroup each, beside all of the above
+  std::vector<PromptItem> prompts;   // scored: units of long segments, a workgroup each, beside all of the above
 };
 
 // Segments of at least this many rows run on the matrix-core prefill kernel by default (Metal's

@@ -107,7 +107,7 @@ __device__ __forceinline__ void redo(const PageGeom& g, const UnitGeom& u, const
 // branch's values ahead of the test).
 template <int KVT, int HD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : 2, HD == 64 ? 4 : 2)))
-void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillItem* items, const float* q, float* out, MergeCopy mc) {
+void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem* items, const float* q, float* out, MergeCopy mc) {
   using C = Shape<KVT, HD>;
   constexpr bool Q8 = C::Q8, BF = C::BF;
   constexpr int NCB = C::NCB, COLS = C::COLS, NC = C::NC, NJ = C::NJ, NI = C::NI;
@@ -117,10 +117,10 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PrefillIte
   const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t hq = lane & 15u, grp = lane >> 4, G = u.group;
   // the unit's record: one load, a word per lane, broadcast to scalar registers
-  const uint32_t word = lane < sizeof(PrefillItem) / 4 ? ((const uint32_t*)(items + blockIdx.x))[lane] : 0u;
+  const uint32_t word = lane < sizeof(PromptItem) / 4 ? ((const uint32_t*)(items + blockIdx.x))[lane] : 0u;
   auto fld = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)word, i); };
-  const uint32_t seq = fld(0), kvh = fld(1), row0 = fld(2), pos0 = fld(3), c_off = fld(5), n_col = fld(6), page0 = fld(7),
-                 n_pages = fld(8), slot = fld(9), stride = fld(10);
+  const uint32_t seq = fld(0), kvh = fld(1), row0 = fld(2), pos0 = fld(3), c_off = fld(4), n_col = fld(5), page0 = fld(6),
+                 n_pages = fld(7), slot = fld(8), stride = fld(9);
   const uint32_t page_end = page0 + n_pages, n_tiles = (n_pages + 3) / 4;
 
   // ---- page tiles of a staged item: item i of wave w is a K item (two chunk rows of a page tile; q8_0: a row of codes)
@@ -588,7 +588,7 @@ uint32_t scored_prompt_cols(uint32_t kv_type, uint32_t hd, uint32_t hdv, uint32_
   return n;
 }
 
-hipError_t launch_scored_prompts(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, const PrefillItem* items, uint32_t n_items,
+hipError_t launch_scored_prompts(const PageGeom& g, const UnitGeom& u, const ScoreGeom& sc, const PromptItem* items, uint32_t n_items,
                                  const float* q, float* out, const MergeCopy& mc, hipStream_t s, const LaunchEv& ev) {
   if (n_items == 0) return hipSuccess;
   hipError_t e = hipErrorInvalidValue;

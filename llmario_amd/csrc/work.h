@@ -82,6 +82,14 @@ struct PrefillItem {
   uint32_t blk[8];
 };
 
+// One unit of a long segment with shaped scores (scored_prompt.hip), a workgroup each: a PrefillItem's columns and pages.
+struct PromptItem {
+  uint32_t seq, kvh, row0, pos0;
+  uint32_t c_off, n_col;
+  uint32_t page0, n_pages;
+  uint32_t slot, slot_stride;
+};
+
 // One wave of a unit launch (units.hip): up to 16 or 32 columns of one segment and KV head, as a
 // PrefillItem's, over key pages page0 .. page0 + n_pages - 1: this wave's share of the unit's pages.
 // slot: as a PrefillItem's. blk: the block ids of the wave's first two pages (the last repeated).

@@ -29,7 +29,7 @@ def scored_plan(kv, geo, bt, table, segs, lo, hi, window=0, n_cu=256, per_cu=8, 
     if rc != N.OK and not (c.n_waves or n_items.value or n_prompts.value):
         return rc, None, None, None, None, c
     waves, items = np.zeros((c.n_waves, 10), np.uint32), np.zeros((n_items.value, 8), np.uint32)
-    prompts = np.zeros((n_prompts.value, 20), np.uint32)
+    prompts = np.zeros((n_prompts.value, 10), np.uint32)
     merges = np.zeros((c.n_merges, 6), np.uint32)
     at = lambda a: a.ctypes.data_as(C.c_void_p)
     rc = N.lib().lmh_plan_scored(C.byref(d), arr, len(segs), lo_p, hi_p, per_cu, at(waves), len(waves), at(items), len(items),
@@ -83,10 +83,10 @@ def check(kv, geo, bt, table, segs, lo, hi, window, waves, items, prompts, merge
                 slots.setdefault((t, h), []).append(slot + (col // group) * k)
         at += n
     cols = 256 if geo[2] == 128 else 128
-    assert all(int(a[8]) + 3 >= int(b[8]) for a, b in zip(prompts, prompts[1:]))   # the longest first (in 64-key tiles)
+    assert all(int(a[7]) + 3 >= int(b[7]) for a, b in zip(prompts, prompts[1:]))   # the longest first (in 64-key tiles)
     for u in prompts:
-        seq, kvh, row0, pos0, n_tok, c_off, n_col, page0, n_pages, slot, k, _ = (int(x) for x in u[:12])
-        assert 0 < n_col <= cols and n_pages > 0 and (k > 1) == (slot != NO_SLOT) and n_tok == (c_off + n_col - 1) // group + 1
+        seq, kvh, row0, pos0, c_off, n_col, page0, n_pages, slot, k = (int(x) for x in u)
+        assert 0 < n_col <= cols and n_pages > 0 and (k > 1) == (slot != NO_SLOT)
         assert all(table[seq, p * 16 // bt] >= 0 for p in (page0, page0 + n_pages - 1))
         for col in range(c_off, c_off + n_col):
             t, h = row0 + col // group, kvh * group + col % group
@@ -178,7 +178,7 @@ def test_units_walk_their_documents_only():
     table = contiguous_table([8192], 16)
     rc, waves, _, prompts, _, c = scored_plan("f16", (16, 4, 64, 64), 16, table, [(0, 0, 8192, 0)], list(r.lo), list(r.hi))
     assert rc == N.OK and len(waves) == 0 and len(prompts) == 4 * 8192 // 32   # 128 columns of a group of 4: 32 rows a unit
-    assert int(prompts[:, 8].sum()) == 4 * 16 * sum(2 * (i + 1) for i in range(16))
+    assert int(prompts[:, 7].sum()) == 4 * 16 * sum(2 * (i + 1) for i in range(16))
 
 
 def test_refused_ranges():
