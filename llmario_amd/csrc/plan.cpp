@@ -197,7 +197,9 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
   // waves fit if units may be cut into key pieces wherever a workgroup ends (c_cut; their partials
   // merge in a launch of their own), and the smallest whose whole units pack into the workgroups
   // (c_whole). Cutting has to save more than the merge launch costs.
-  const uint32_t c_min = 4 / KT;
+  // (shaped scores on f32 pages, whose decode rows run here too: from one step; 8 heads of 64, one row of 256 keys
+  // 12.8 -> 10.7 us, of 1,024 19.3 -> 15.1)
+  const uint32_t c_min = in.scored && f32 ? 1 : 4 / KT;
   const uint32_t slack = f32 ? 6 : 3;   // steps: the merge launch's ~4.5 us at ~1.5 us (a 16-key f32 step: 0.8 us)
   const bool cut_ok = !in.prefill_no_split && in.hdv <= 256 && in.hdv % 4 == 0;
   auto smallest = [&](auto&& fits) {
