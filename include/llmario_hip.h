@@ -244,7 +244,8 @@ int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint6
  * rot_dim / 2); with LMH_ROPE_AXES_INTERLEAVED the axes take turns, a = i mod n_axes, axes from 1 on for
  * sections[a] turns (a + n_axes * (sections[a] - 1) < rot_dim / 2) and axis 0 every other pair. With
  * LMH_ROPE_AXES_OWN_FREQ each axis has frequencies of its own: pair j of its n pairs has theta^(-j/n). Everything
- * else as lmh_qk_rope_store, whose flags must hold LMH_ROPE_APPLY. */
+ * else as lmh_qk_rope_store, whose flags must hold LMH_ROPE_APPLY. A stream under graph capture is refused with
+ * LMH_UNSUPPORTED (the call's lists sit in a staging slot that later calls reuse). */
 #define LMH_ROPE_AXES_INTERLEAVED 1u
 #define LMH_ROPE_AXES_OWN_FREQ 2u
 typedef struct lmh_rope_axes {

@@ -22,6 +22,7 @@
 #include <cstring>
 #include <map>
 #include <queue>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -754,6 +755,20 @@ void kv_detach(lmh_kv* kv, lmh_sched* s) {
 }
 }  // namespace lmh
 
+// A call's body behind the C boundary: an exception (a host list that finds no memory) ends as a status.
+template <typename F>
+static int32_t guarded(lmh_kv* kv, F&& body) noexcept {
+  try {
+    return body();
+  } catch (const std::bad_alloc&) {
+    if (kv) kv->err = "host memory";   // (short: held in the string itself)
+    return LMH_OUT_OF_MEMORY;
+  } catch (...) {
+    if (kv) kv->err = "host error";
+    return LMH_DEVICE_ERROR;
+  }
+}
+
 extern "C" {
 
 const char* lmh_create_error(void) { return g_create_error.c_str(); }
@@ -1379,11 +1394,11 @@ int32_t lmh_kv_store_encoded(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, ui
 }
 int32_t lmh_kv_gather(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, float* k, float* v,
                       void* stream) {
-  return kv_io(kv, layer, segs, n_segs, k, v, stream, 2);
+  return guarded(kv, [&] { return kv_io(kv, layer, segs, n_segs, k, v, stream, 2); });
 }
 int32_t lmh_kv_gather_encoded(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, void* k, void* v,
                               void* stream) {
-  return kv_io(kv, layer, segs, n_segs, k, v, stream, 3);
+  return guarded(kv, [&] { return kv_io(kv, layer, segs, n_segs, k, v, stream, 3); });
 }
 
 // What is wrong with the axes of a call with `half` rotated pairs, or nullptr.
@@ -1423,6 +1438,14 @@ static void axes_turns(const lmh_rope_axes* x, const lmh_rope_params* p, double*
     seen[a]++;
     turns[i] = (double)p->freq_scale * std::pow((double)p->theta, e) * 0.15915494309189533577;
   }
+}
+
+static int32_t refuse_capture(lmh_kv* kv, void* stream, const char* name) {
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing((hipStream_t)stream, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone)
+    return kv->fail(LMH_UNSUPPORTED, std::string(name) + " cannot be captured into a graph: its work list lives in a "
+                                                         "staging slot that later calls reuse");
+  return LMH_OK;
 }
 
 static int32_t rope_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
@@ -1521,15 +1544,18 @@ static int32_t rope_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64
 int32_t lmh_qk_rope_store(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
                           const float* k_in, const float* v_in, float* q_out, const lmh_rope_params* p,
                           void* stream) {
-  return rope_impl(kv, layer, segs, n_segs, q_in, k_in, v_in, q_out, p, nullptr, stream);
+  return guarded(kv, [&] { return rope_impl(kv, layer, segs, n_segs, q_in, k_in, v_in, q_out, p, nullptr, stream); });
 }
 
 int32_t lmh_qk_rope_store_axes(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q_in,
                                const float* k_in, const float* v_in, float* q_out, const lmh_rope_params* p,
                                const lmh_rope_axes* axes, void* stream) {
   if (!kv) return LMH_INVALID_ARGUMENT;
-  if (!axes) return kv->fail(LMH_INVALID_ARGUMENT, "rope axes: null");
-  return rope_impl(kv, layer, segs, n_segs, q_in, k_in, v_in, q_out, p, axes, stream);
+  return guarded(kv, [&]() -> int32_t {
+    if (!axes) return kv->fail(LMH_INVALID_ARGUMENT, "rope axes: null");
+    if (const int32_t rc = refuse_capture(kv, stream, "lmh_qk_rope_store_axes"); rc != LMH_OK) return rc;
+    return rope_impl(kv, layer, segs, n_segs, q_in, k_in, v_in, q_out, p, axes, stream);
+  });
 }
 
 // What the planner needs to know of the kernel modules for a layer's geometry.
@@ -1580,17 +1606,11 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
                            float* out, float scale, uint64_t window, void* stream, bool noalloc,
                            const lmh_score_params* sp = nullptr) {
   if (!kv) return LMH_INVALID_ARGUMENT;
-  const char* const name = sp ? "lmh_attend_scored" : "lmh_attend";
   if (noalloc && !kv->scratch) return kv->fail(LMH_DEVICE_ERROR, "no-allocation scratch not resolved");
   // A captured graph would replay this call's kernels against a staging slot that later calls
   // overwrite (the work list is read from it when the kernels run), so capture is refused before
   // anything is enqueued.
-  {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing((hipStream_t)stream, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone)
-      return kv->fail(LMH_UNSUPPORTED, std::string(name) + " cannot be captured into a graph: its work list lives in a "
-                                                            "staging slot that later calls reuse");
-  }
+  if (const int32_t rc = refuse_capture(kv, stream, sp ? "lmh_attend_scored" : "lmh_attend"); rc != LMH_OK) return rc;
   if (layer >= kv->layers.size()) return kv->fail(LMH_INVALID_ARGUMENT, "layer out of range");
   if (!std::isfinite(scale)) return kv->fail(LMH_INVALID_ARGUMENT, "scale must be finite");
   uint64_t n_rows;
@@ -1802,25 +1822,27 @@ static int32_t attend_impl(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint
 
 int32_t lmh_attend(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q, float* out,
                    float scale, uint64_t window, void* stream) {
-  return attend_impl(kv, layer, segs, n_segs, q, out, scale, window, stream, false);
+  return guarded(kv, [&] { return attend_impl(kv, layer, segs, n_segs, q, out, scale, window, stream, false); });
 }
 
 int32_t lmh_attend_noalloc(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q,
                            float* out, float scale, uint64_t window, void* stream) {
-  return attend_impl(kv, layer, segs, n_segs, q, out, scale, window, stream, true);
+  return guarded(kv, [&] { return attend_impl(kv, layer, segs, n_segs, q, out, scale, window, stream, true); });
 }
 
 int32_t lmh_attend_scored(lmh_kv* kv, uint32_t layer, const lmh_seg* segs, uint64_t n_segs, const float* q, float* out,
                           const lmh_score_params* p, void* stream) {
   if (!kv) return LMH_INVALID_ARGUMENT;
-  if (!p || p->abi_version != LMH_ABI_VERSION) return kv->fail(LMH_INVALID_ARGUMENT, "score params: null or ABI version");
-  if (p->reserved0) return kv->fail(LMH_INVALID_ARGUMENT, "score params: reserved0 must be 0");
-  if (!(p->cap >= 0.f) || !std::isfinite(p->cap)) return kv->fail(LMH_INVALID_ARGUMENT, "cap must be finite and not negative");
-  // (scale: tested with the call's other arguments)
-  if (p->cap > 0.f && std::isfinite(p->scale) && (!std::isfinite(p->scale / p->cap) || !std::isfinite(p->cap * 1.4426950408889634f)))
-    return kv->fail(LMH_INVALID_ARGUMENT, "scale / cap is out of range");
-  if ((uintptr_t)p->slopes % 4) return kv->fail(LMH_INVALID_ARGUMENT, "slopes must be 4-byte aligned");
-  return attend_impl(kv, layer, segs, n_segs, q, out, p->scale, p->window, stream, false, p);
+  return guarded(kv, [&]() -> int32_t {
+    if (!p || p->abi_version != LMH_ABI_VERSION) return kv->fail(LMH_INVALID_ARGUMENT, "score params: null or ABI version");
+    if (p->reserved0) return kv->fail(LMH_INVALID_ARGUMENT, "score params: reserved0 must be 0");
+    if (!(p->cap >= 0.f) || !std::isfinite(p->cap)) return kv->fail(LMH_INVALID_ARGUMENT, "cap must be finite and not negative");
+    // (scale: tested with the call's other arguments)
+    if (p->cap > 0.f && std::isfinite(p->scale) && (!std::isfinite(p->scale / p->cap) || !std::isfinite(p->cap * 1.4426950408889634f)))
+      return kv->fail(LMH_INVALID_ARGUMENT, "scale / cap is out of range");
+    if ((uintptr_t)p->slopes % 4) return kv->fail(LMH_INVALID_ARGUMENT, "slopes must be 4-byte aligned");
+    return attend_impl(kv, layer, segs, n_segs, q, out, p->scale, p->window, stream, false, p);
+  });
 }
 
 // nullptr, or what is wrong with the options
@@ -1984,20 +2006,22 @@ int32_t lmh_plan_scored(const lmh_plan_desc* d, const lmh_seg* segs, uint64_t n_
                         uint64_t items_cap, uint32_t* prompts, uint64_t prompts_cap, uint32_t* merges, uint64_t merges_cap,
                         lmh_plan_wave_counts* counts, uint64_t* n_items, uint64_t* n_prompts) {
   if (!counts || !n_items || !n_prompts || waves_per_cu == 0) return LMH_INVALID_ARGUMENT;
-  PlanIn in;
-  PlanOut o;
-  in.unit_waves_given = waves_per_cu;
-  if (const int32_t rc = plan_desc(d, segs, n_segs, in, o, true, row_lo, row_hi); rc != LMH_OK) return rc;
-  *counts = lmh_plan_wave_counts{o.uwaves.size(), o.merges.size(), sizeof(UnitWave) / 4, sizeof(MergeItem) / 4,
-                                 o.u_w, o.u_nb, o.u_shared ? 1u : 0u, o.ng, o.slots, in.layout};
-  *n_items = o.items.size();
-  *n_prompts = o.prompts.size();
-  if (o.uwaves.size() > waves_cap || o.items.size() > items_cap || o.prompts.size() > prompts_cap || o.merges.size() > merges_cap) return LMH_INVALID_ARGUMENT;
-  if (!o.uwaves.empty()) std::memcpy(waves, o.uwaves.data(), o.uwaves.size() * sizeof(UnitWave));
-  if (!o.items.empty()) std::memcpy(items, o.items.data(), o.items.size() * sizeof(DecodeItem));
-  if (!o.prompts.empty()) std::memcpy(prompts, o.prompts.data(), o.prompts.size() * sizeof(PromptItem));
-  if (!o.merges.empty()) std::memcpy(merges, o.merges.data(), o.merges.size() * sizeof(MergeItem));
-  return LMH_OK;
+  return guarded(nullptr, [&]() -> int32_t {
+    PlanIn in;
+    PlanOut o;
+    in.unit_waves_given = waves_per_cu;
+    if (const int32_t rc = plan_desc(d, segs, n_segs, in, o, true, row_lo, row_hi); rc != LMH_OK) return rc;
+    *counts = lmh_plan_wave_counts{o.uwaves.size(), o.merges.size(), sizeof(UnitWave) / 4, sizeof(MergeItem) / 4,
+                                   o.u_w, o.u_nb, o.u_shared ? 1u : 0u, o.ng, o.slots, in.layout};
+    *n_items = o.items.size();
+    *n_prompts = o.prompts.size();
+    if (o.uwaves.size() > waves_cap || o.items.size() > items_cap || o.prompts.size() > prompts_cap || o.merges.size() > merges_cap) return LMH_INVALID_ARGUMENT;
+    if (!o.uwaves.empty()) std::memcpy(waves, o.uwaves.data(), o.uwaves.size() * sizeof(UnitWave));
+    if (!o.items.empty()) std::memcpy(items, o.items.data(), o.items.size() * sizeof(DecodeItem));
+    if (!o.prompts.empty()) std::memcpy(prompts, o.prompts.data(), o.prompts.size() * sizeof(PromptItem));
+    if (!o.merges.empty()) std::memcpy(merges, o.merges.data(), o.merges.size() * sizeof(MergeItem));
+    return LMH_OK;
+  });
 }
 
 int32_t lmh_bench_read_ceiling(int32_t device, uint64_t bytes, uint32_t iters, double* gbps) {

@@ -658,16 +658,17 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
           if (in.segs[i].n > 0) longer.push_back((uint32_t)i);
         rest.clear();
       } else if (of_long * in.n_kv <= 3ull * in.n_cu) {   // and the other way round
-        plan_units(in, o);
-        return;
+        if (plan_units(in, o)) return;
       }
       plan_prompts(in, longer, o);
       if (rest.empty()) return;
       PlanIn less = in;
       less.segs = rest.data();
       less.n_segs = rest.size();
-      plan_units(less, o);   // every geometry with an instance above has one there
-      return;
+      if (plan_units(less, o)) return;   // (every geometry with an instance above has one there)
+      o.prompts.clear();
+      o.merges.clear();
+      o.slots = 0;
     }
   }
   if (plan_units(in, o)) return;

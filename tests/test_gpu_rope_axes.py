@@ -192,6 +192,40 @@ def test_refusals():
         assert call(axes(**kw)) == N.INVALID_ARGUMENT, kw
 
 
+def test_capture_is_refused():
+    hc = HipKvCache([Layer(8, 2, 128, 128)], max_ctx=64, n_seqs=1, kv_type="f16")
+    hc.reserve(0, 4)
+    q, k, v = (torch.randn(4, h, 128, device="cuda") for h in (8, 2, 2))
+    out, pos = torch.zeros_like(q), torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+    hc.qk_rope_store_axes(0, [(0, 0, 4, 0)], q, k, v, out, pos, [24, 20, 20])
+    torch.cuda.synchronize()
+    refused = None
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            hc.qk_rope_store_axes(0, [(0, 0, 4, 0)], q, k, v, out, pos, [24, 20, 20])
+        except LmhError as e:
+            refused = e.status
+        out.add_(0.0)
+    assert refused == N.UNSUPPORTED
+
+
+def test_another_rotation_after_one_and_back():
+    """The table of turns kept from the latest call is not another rotation's."""
+    hc = HipKvCache([Layer(8, 2, 128, 128)], max_ctx=64, n_seqs=1, kv_type="f32")
+    hc.reserve(0, 40)
+    q, k, v = (torch.randn(40, h, 128, device="cuda") for h in (8, 2, 2))
+    pos = torch.randint(0, 500, (3, 40), dtype=torch.int32, device="cuda")
+    outs = []
+    for kw in ({}, {"theta": 1e6}, {"freq_scale": 0.5}, {"rot_dim": 64, "sections": [12, 10, 10]}, {"interleaved": True, "sections": [22, 21, 21]},
+               {"sections": [20, 22, 22]}, {"own_freq": True}, {}):
+        out = torch.empty_like(q)
+        hc.qk_rope_store_axes(0, [(0, 0, 40, 0)], q, k, v, out, pos, **{"sections": [24, 20, 20], **kw})
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[-1])
+    assert all(not torch.equal(outs[0], o) for o in outs[1:-1])
+
+
 @pytest.mark.parametrize("kv", ["f16", "bf16", "f32"])
 def test_an_image_prompt_and_its_answer(kv):
     """Both operators as a layer runs them: a prompt of text and an image (positions of three axes, the prefix's tokens

@@ -39,7 +39,7 @@ def test_forms(form, kind):
     c = Call(kv, geo, prior, new, bt, seed=11)
     r, sl = ranges_of(kind, c.segs, seed=12), slopes_of(geo[0])
     rows = None if max(new) < 70 else sorted({0, 1, 2, 31, 32, 33, 63, 64, 65, 127, max(new) - 2, max(new) - 1})
-    for kw in ({}, {"cap": 2.0, "slopes": sl}, {"cap": 40.0}):
+    for kw in ({}, {"cap": 2.0, "slopes": sl}, {"cap": 40.0}, {"slopes": sl}):
         kw = dict(kw, window=window, ranges=r)
         c.check(c.run(**kw), rows=rows, **kw)
 
@@ -61,6 +61,35 @@ def test_chunks_on_long_prefixes_in_pieces(kv, geo, prior, new):
             hi.append(b)
     r = RowRanges(lo, hi)
     c.check(c.run(cap=20.0, ranges=r), cap=20.0, ranges=r, rows=rows)
+
+
+@pytest.mark.parametrize("kv,hd", [("f16", 64), ("bf16", 128), ("q8_0", 128), ("f16", 256)])
+def test_scales_of_any_sign(kv, hd):
+    c = Call(kv, (8, 2, hd, hd), [50], [70], seed=21, spread=4.0)
+    for kw in ({"scale": -0.1}, {"scale": 0.0}, {"scale": -0.2, "cap": 3.0}, {"scale": 0.0, "slopes": slopes_of(8)},
+               {"scale": 1.0, "cap": 1e-2}, {"scale": 0.02, "cap": 1e20}):
+        c.check(c.run(**kw), rows=[0, 1, 33, 69], **kw)
+
+
+@pytest.mark.parametrize("kv,geo", [("bf16", (32, 8, 128, 128)), ("f16", (8, 2, 64, 64)), ("q8_0", (16, 4, 128, 128))])
+def test_pieces_that_hold_values_that_are_not_finite(kv, geo):
+    """A unit cut into key pieces, one of which holds a key of V beyond any number: the rows that do not see it."""
+    c = Call(kv, geo, [5000], [40], seed=22)
+    lo = [0 if j % 2 else 2001 for j in range(40)]
+    r = RowRanges(lo, None)
+    clean = c.run(slopes=slopes_of(geo[0], 2.0 ** -9), ranges=r).clone()
+    c.hc.store(0, [(0, 0, 1, 2000)], c.k[0][2000:2001].contiguous(), torch.full_like(c.v[0][:1], 3e38 if kv == "q8_0" else float("inf")))
+    out = c.run(slopes=slopes_of(geo[0], 2.0 ** -9), ranges=r)
+    assert torch.isfinite(out[0::2]).all() and not torch.isfinite(out[1::2]).any()
+    assert (out[0::2] - clean[0::2]).abs().max().item() <= 1e-4
+
+
+def test_short_segments_beside_long_ones():
+    """Decode rows in the prompts' launch, in one of their own before it, and a short prompt in theirs: the same rows."""
+    for prior, new in (([300, 40, 7, 0], [1, 1, 2, 500]), ([3000] * 20 + [0], [1] * 20 + [150]), ([5000] * 24 + [0, 64], [1] * 24 + [600, 300])):
+        for kv, geo in (("bf16", (16, 4, 128, 128)), ("f16", (8, 2, 64, 64))):
+            c = Call(kv, geo, prior, new, seed=23)
+            c.check(c.run(cap=10.0), cap=10.0, rows=[0, 1, 140, 499])
 
 
 def refill(c, s, k_mul=1.0, v_mul=1.0, from_pos=0):
