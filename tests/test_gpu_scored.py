@@ -175,6 +175,22 @@ def test_scores_and_ranges(form, kind):
             c.check(c.run(**kw), **kw)
 
 
+WIDTHS = [(kv, hd, hdv) for kv in ("f16", "bf16") for hd, hdv in ((32, 32), (64, 64), (96, 96), (128, 128), (192, 192), (256, 256), (192, 128),
+                                                                   (40, 40), (80, 80), (120, 112), (160, 160), (240, 256))] + \
+    [("q8_0", d, d) for d in (64, 128, 192, 256)] + [("f32", d, d) for d in (60, 128, 200)]
+
+
+@pytest.mark.parametrize("new", [1, 15])
+@pytest.mark.parametrize("kv,hd,hdv", WIDTHS)
+def test_every_width(kv, hd, hdv, new):
+    """One column block (a decode row) and two (a run of drafted tokens) of every instance."""
+    c = Call(kv, (8, 2, hd, hdv), [83, 5], [new, new], seed=31)
+    r = ranges_of("random", c.segs, seed=32)
+    sl = slopes_of(8)
+    c.check(c.run(cap=6.0, slopes=sl), cap=6.0, slopes=sl)
+    c.check(c.run(ranges=r), ranges=r)
+
+
 @pytest.mark.parametrize("kind", ["one", "none"])
 @pytest.mark.parametrize("form", FORMS, ids=IDS)
 def test_rows_that_see_one_key_or_none(form, kind):
