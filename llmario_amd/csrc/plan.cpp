@@ -200,7 +200,10 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
   // (shaped scores on f32 pages, whose decode rows run here too: from one step; 8 heads of 64, one row of 256 keys
   // 12.8 -> 10.7 us, of 1,024 19.3 -> 15.1)
   const uint32_t c_min = in.scored && f32 ? 1 : 4 / KT;
-  const uint32_t slack = f32 ? 6 : 3;   // steps: the merge launch's ~4.5 us at ~1.5 us (a 16-key f32 step: 0.8 us)
+  // steps: the merge launch's ~4.5 us at ~1.5 us (a 16-key f32 step: 0.8 us). Shaped scores, whose decode rows run here
+  // too with waves to spare, at 3, 5 and 8 steps, us: 32 q8_0 rows of 512 .. 4,096 keys 38.5, 37.0, 44.4; 48 bf16 rows of
+  // documents 34.0, 32.1, 32.2; 120 rows of a prompt beside 8 decode rows, heads of 80, 32.8, 26.9, 27.5.
+  const uint32_t slack = f32 ? 6 : in.scored ? 5 : 3;
   const bool cut_ok = !in.prefill_no_split && in.hdv <= 256 && in.hdv % 4 == 0;
   auto smallest = [&](auto&& fits) {
     uint32_t lo = (uint32_t)std::max<uint64_t>(c_min, (total + target - 1) / target), hi = std::max<uint32_t>(lo, (uint32_t)max_ns);
@@ -485,8 +488,8 @@ bool plan_units(const PlanIn& in, PlanOut& o) {
 
 // Segments of at least this many columns (rows x query heads of a KV head) run on the kernel for long segments. 8
 // sequences on 2,000 keys, 32/8 heads of 128, bf16, us: 4 rows each 33.1 so, 27.0 in the unit launch; 16 36.6 and 38.0; 32
-// 42.9 and 43.7; q8_0 32 rows 49.0 and 50.9, 16 42.2 and 41.2; 32 sequences of 16 rows 86.5 and 85.0, q8_0 108 and 87; one
-// prompt of 2,048 a fourth of the unit launch's time less a third.
+// 42.9 and 43.7; q8_0 32 rows 49.0 and 50.9, 16 42.2 and 41.2; 32 sequences of 16 rows 86.5 and 85.0, q8_0 108 and 87;
+// four prompts of 2,048 370 here and 627 there.
 constexpr uint64_t PROMPT_MIN_COLS = 128;
 // A unit's fixed cost (its Q, the first tile's way through LDS, its stores) and that of a merge launch, in 64-key tiles
 // (~3.5 us of a workgroup at 256 columns; half that on heads of 64). Two prompts of 700 rows, us, whole / in pieces: q8_0
@@ -637,7 +640,7 @@ void plan_attend(const PlanIn& in, PlanOut& o) {
     if (!longer.empty()) {
       // Few short segments go along, a workgroup each, rather than in a launch of their own (~10 us and its share of the
       // merge): while they take the device less than that, or than an eighth of the long ones' time. (4 decode rows beside two prompts of ~850 rows,
-      // window 1,024, 16/4 heads of 256: 71 us in two launches, 62 in one.)
+      // window 1,024, 16/4 heads of 256: 71 us in two launches, 59 in one.)
       auto tiles_of = [&](const lmh_seg& sg) -> uint64_t {
         uint64_t n = 0;
         const uint64_t cols = sg.n * group;
