@@ -12,8 +12,12 @@
 //   O^T[dims x cols] += V^T . P^T    v_mfma_f32_16x16x32_f16, weights as f16 hi + lo parts
 // (q8_0: K hi . Q hi + K hi . Q lo + K lo . Q hi, and V likewise.) f16 has less range than bf16 or a scaled code: K
 // and V are scaled by powers of two taken from the largest magnitude of the unit's first tile when that lies outside
-// 2^-6 .. 2^8, and a unit whose K leaves f16's range later, or whose outputs are not finite (a NaN or an infinity in
-// V, seen or not), is computed again on the vector units in f32 (redo), straight from the pages.
+// 2^0 .. 2^8 (q8_0, whose small products are multiples of 2^-24 and so exact: 2^-6 .. 2^8), to 2^3 .. 2^4. Computed again
+// on the vector units in f32, straight from the pages (redo): all columns of a unit whose K leaves f16's range later;
+// columns whose outputs are not finite (a NaN or an infinity in V, seen or not); and columns whose outputs are so small
+// that V's rounding below 2^-17 (bf16; half a step, 2^-25) could be seen in them: n keys, a largest output M with
+// M sqrt(n) < 2^-5 (V of their keys 2^-5 and less of the first tile's). K's rounding there is not looked for: it moves a
+// score by 2^-25 of what the first tile's keys score.
 //
 // Per tile: the next tile's pages are requested into registers, the tile in LDS is multiplied, then the registers are
 // expanded into the other LDS buffer and one barrier publishes it.
@@ -112,7 +116,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
   constexpr bool Q8 = C::Q8, BF = C::BF;
   constexpr int NCB = C::NCB, COLS = C::COLS, NC = C::NC, NJ = C::NJ, NI = C::NI;
   extern __shared__ __attribute__((aligned(16))) uint8_t prompt_lds[];
-  uint32_t* words = (uint32_t*)(prompt_lds + 2 * C::STAGE);   // [8] K maxima, [8] V maxima, [16] the redo flag
+  uint32_t* words = (uint32_t*)(prompt_lds + 2 * C::STAGE);   // [8] K maxima, [8] V maxima, [16] the redo flag, [17] some V is not 0
   copy_merges(mc, blockIdx.x, gridDim.x);
   const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t hq = lane & 15u, grp = lane >> 4, G = u.group;
@@ -250,7 +254,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
   // ---- the powers of two of K and V (bf16, q8_0), from the first tile
   float k_mul = 1.f, v_mul = 1.f;
   int v_exp = 0;
-  if (threadIdx.x == 0) words[16] = 0;
+  if (threadIdx.x == 0) words[16] = words[17] = 0;
   if constexpr (BF || Q8) {
     uint32_t top[2] = {0, 0};
 #pragma unroll
@@ -296,7 +300,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       const float f = Q8 ? h_to_f((uint16_t)bits) * 127.0f : __uint_as_float(bits << 16);
       if (!(f < INFINITY) || f == 0.f) return 0;
       const int e = __builtin_amdgcn_frexp_expf(f);
-      return e >= -6 && e <= 8 ? 0 : min(max(e, -120), 120);
+      return e >= (Q8 ? -6 : 1) && e <= 8 ? 0 : min(max(e - 4, -120), 120);
     };
     const int ke = __builtin_amdgcn_readfirstlane(exponent(km));
     v_exp = __builtin_amdgcn_readfirstlane(exponent(vm));
@@ -310,6 +314,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   typedef float f2 __attribute__((ext_vector_type(2)));
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  uint32_t v_bits = 0;   // of all V written by this lane (bf16)
   u16x2 k_top = 0;   // largest |K| bits written by this lane (bf16, q8_0): 0x7c00 and more left f16's range
   const bool plain = k_mul == 1.f && v_mul == 1.f;   // uniform
   auto widen = [&](uint32_t x, float mul) -> uint32_t {   // two bf16
@@ -381,6 +386,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       } else {           // [4 keys of dim d | of dim d + 16] of both tiles into blocks 2b and 2b + 1 of 8 keys
         uint4 a = raw[i][0], b = raw[i][1];
         if constexpr (BF) {
+          v_bits |= (a.x | a.y | a.z) | (a.w | b.x | b.y) | (b.z | b.w);
           a = widen4(a, v_mul);
           b = widen4(b, v_mul);
         }
@@ -515,25 +521,45 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
   // ---- results
   if constexpr (BF || Q8) {
     if (max(k_top[0], k_top[1]) >= 0x7c00) words[16] = 1;
+    if (BF && (v_bits & 0x7fff7fffu)) words[17] = 1;
     __syncthreads();
   }
-  bool bad = (BF || Q8) && words[16] != 0;
+  const bool all = (BF || Q8) && words[16] != 0, lossy = BF ? words[17] != 0 : Q8 && v_mul < 1.f;
+  bool bad[NCB], some = false;
 #pragma unroll
   for (int x = 0; x < NCB; x++) {
     lsum[x] = xsum_groups(lsum[x]);
     float z = lsum[x];
 #pragma unroll
     for (int j = 0; j < NJ; j++) z += (O[x][j][0] + O[x][j][1]) + (O[x][j][2] + O[x][j][3]);
-    bad |= cv[x] && !__builtin_isfinite(z);
+    bad[x] = all || !__builtin_isfinite(z);
+    if (lossy) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) top = fmaxf(top, fmaxf(fmaxf(fabsf(O[x][j][0]), fabsf(O[x][j][1])), fmaxf(fabsf(O[x][j][2]), fabsf(O[x][j][3]))));
+      top = xmax_groups(top);
+      bad[x] |= top * top * (float)min(clen[x], n_pages << 4) < lsum[x] * lsum[x] * 0x1p-10f;
+    }
+    bad[x] &= cv[x];
+    some |= bad[x];
   }
   auto row_at = [&](uint32_t tok, uint32_t head) -> float* {
     if (slot == NO_SLOT) return out + ((size_t)(row0 + tok) * u.n_head + (size_t)kvh * G + head) * HD;
     return u.part + ((size_t)(slot + tok * stride) * u.ng + head) * (HD + 4);
   };
-  if (__builtin_expect(__ballot(bad) != 0, 0)) {
+  if (__builtin_expect(__ballot(some) != 0, 0)) {
+    uint32_t again = 0;   // a bit per column of the wave
+#pragma unroll
+    for (int x = 0; x < NCB; x++) {
+      uint64_t b = __ballot(bad[x]);
+      b |= b >> 32;
+      b |= b >> 16;
+      again |= ((uint32_t)b & 0xffffu) << (16 * x);
+      cv[x] = cv[x] && !(again >> (16 * x + hq) & 1u);
+    }
 #pragma clang loop unroll(disable)
-    for (uint32_t c = 0; c < (uint32_t)COLS && w * COLS + c < n_col; c++) {
-      const uint32_t a = w * COLS + c + c_off, tok = a / G, head = a - tok * G, pos = pos0 + tok;
+    for (; again; again &= again - 1) {
+      const uint32_t a = w * COLS + (uint32_t)__builtin_ctz(again) + c_off, tok = a / G, head = a - tok * G, pos = pos0 + tok;
       uint32_t first = (u.window > 0 && pos + 1 > u.window) ? pos + 1 - u.window : 0, last = pos;
       if (sc.ranges) {
         const uint2 r = sc.ranges[row0 + tok];
@@ -545,7 +571,6 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       redo<KVT, HD>(g, u, sc, seq, kvh, kvh * G + head, pos, first, end,
                     q + ((size_t)(row0 + tok) * u.n_head + (size_t)kvh * G + head) * HD, row_at(tok, head), slot != NO_SLOT);
     }
-    return;
   }
   typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll

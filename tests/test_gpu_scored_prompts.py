@@ -128,6 +128,52 @@ def test_magnitudes_that_grow_along_the_sequence(kv, geo):
         c.check(c.run(cap=15.0), cap=15.0, rows=[0, 1, 30, 89])
 
 
+@pytest.mark.parametrize("mul", [1e-2, 1e-4, 1e-7, 1e2, 1e4])
+@pytest.mark.parametrize("kv,geo", [x for x in SIZES if x[0] != "f16"], ids=[f"{k}-{g[2]}" for k, g in SIZES if k != "f16"])
+def test_documents_of_other_magnitudes(kv, geo, mul):
+    """Packed documents whose V (then K) is far from the first one's: each row within the tolerance of the V it sees."""
+    if kv == "q8_0":
+        mul = min(max(mul, 1e-3), 1e3)   # (its scales are f16: 1e-3 of a row at 1e-1 is held to 2^-10 or so, as read back)
+    for base in (0.1, 1.0, 30.0):
+        c = Call(kv, geo, [0], [190], seed=17)
+        refill(c, 0, 1.0, base)
+        refill(c, 0, 1.0, base * mul, from_pos=70)
+        r = RowRanges.of(c.segs, documents=[[0, 70, 71, 75, 130]])
+        for kw in ({"ranges": r}, {"ranges": r, "cap": 15.0}, {"window": 20}):
+            c.check(c.run(**kw), rows=[0, 5, 69, 70, 71, 72, 75, 80, 129, 130, 131, 189], **kw)
+        refill(c, 0, 1.0, 1.0)
+        refill(c, 0, mul, 1.0, from_pos=70)
+        c.check(c.run(ranges=r), rows=[0, 69, 70, 72, 80, 130, 189], ranges=r)
+
+
+@pytest.mark.parametrize("kv,geo", SIZES, ids=[f"{k}-{g[2]}" for k, g in SIZES])
+def test_a_head_whose_v_is_zero(kv, geo):
+    c = Call(kv, geo, [0], [150], seed=18)
+    c.v[0].view(150, geo[1], geo[3])[:, 0] = 0.0
+    refill(c, 0)
+    out = c.run(cap=15.0)
+    c.check(out, cap=15.0, rows=[0, 1, 64, 149])
+    if geo[1] > 1:
+        assert (out[:, :geo[0] // geo[1]] == 0).all()
+
+
+@pytest.mark.parametrize("mul", [1e-2, 1e-4, 1e-7, 1e2, 1e4])
+@pytest.mark.parametrize("kv,geo", [("bf16", (8, 2, 128, 128)), ("q8_0", (8, 2, 64, 64)), ("bf16", (8, 8, 96, 96)), ("f32", (8, 2, 64, 64)), ("bf16", (4, 2, 80, 80)), ("q8_0", (4, 2, 96, 96))],
+                         ids=lambda x: x if isinstance(x, str) else str(x[2]))
+def test_documents_of_other_magnitudes_in_short_segments(kv, geo, mul):
+    """The same in the unit launch: decode rows and drafted tokens."""
+    if kv == "q8_0":
+        mul = min(max(mul, 1e-3), 1e3)
+    for base in (0.1, 1.0, 30.0):
+        c = Call(kv, geo, [171, 70], [5, 1], seed=17)
+        for s in range(2):
+            refill(c, s, 1.0, base)
+            refill(c, s, 1.0, base * mul, from_pos=50)
+        lo, hi = [0, 50, 100, 49, 52, 50], [50, 51, 175, 52, 70, 71]
+        for kw in ({"ranges": RowRanges(lo, hi)}, {"ranges": RowRanges(lo, hi), "cap": 15.0}, {"window": 20}):
+            c.check(c.run(**kw), **kw)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("form", [f for f in FORMS if f[4] == 16 and not f[5] and f[1][0] < 50], ids=lambda f: f"{f[0]}-{f[1][2]}-{f[3][0]}")
 def test_values_that_are_not_finite(form, bad):
