@@ -43,8 +43,8 @@ def _stream_ptr(stream):
     if isinstance(stream, C.c_void_p):
         return stream
     if stream is None:
-        import torch
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        import torch   # (the stream's address alone: 0.5 us; torch.cuda.current_stream() builds an object, 2.7 us)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
     if isinstance(stream, int):
         return C.c_void_p(stream)
     return C.c_void_p(stream.cuda_stream)
