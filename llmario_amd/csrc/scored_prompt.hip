@@ -21,6 +21,15 @@
 //
 // Per tile: the next tile's pages are requested into registers, the tile in LDS is multiplied, then the registers are
 // expanded into the other LDS buffer and one barrier publishes it.
+//
+// Q and the weights in two parts are two products per pair (q8_0: three), so half (a third) of a large product's
+// 1,260 TFLOP/s is the ceiling. Measured, us, with the share of the matrix pipe and of VALU issue: four prompts of 2,048
+// tokens whose first halves see each other, 32/8 heads of 128, bf16: 370, 525 TFLOP/s, 39 % and 35 % (the unit launch 627; a
+// third LDS buffer with the next tile's scores issued ahead of this one's softmax 406 .. 421); three of 401 .. 2,047 on
+// q8_0 pages with a cap 104, 25 % and 33 %, and units of uneven lengths; 8,192 packed tokens of 16/4 heads of 64, f16, 45,
+// 19 % and 32 %: 1,024 units of few tiles, most of it their way from the record to the first tile; two of 600 .. 1,100 tokens,
+// 16/4 heads of 256, bf16, window 1,024, cap 50, 51 and the pieces' merge 5.5, 13 % and 21 %, one workgroup to a CU.
+// Traffic is small beside that (0.4 .. 1.1 TB/s). No LDS bank conflicts on 16-bit pages; q8_0's 8-byte V stores have a few.
 #include "decode_tile.h"
 #include "score.h"
 
@@ -75,7 +84,7 @@ __device__ __forceinline__ void redo(const PageGeom& g, const UnitGeom& u, const
     const uint8_t* b = g.pool + (size_t)(uint32_t)tab[key >> g.bt_shift] * g.block_bytes;
     const uint8_t* kh = b + g.k_off + (size_t)kvh * g.k_head;
     float s = 0.f;
-#pragma clang loop unroll(disable)
+#pragma clang loop unroll_count(16)
     for (uint32_t d = 0; d < (uint32_t)HD; d++)
       s = fmaf(q[d], page_value<KVT>(kh, (key & bt_mask) >> 4, g.k_tile, g.k_scale, g.k_tile_s, false, key & 15u, d, HD), s);
     float p[1] = {s * u.scale_log2};
@@ -90,7 +99,7 @@ __device__ __forceinline__ void redo(const PageGeom& g, const UnitGeom& u, const
     l = l * alpha + sum;
     m = mn;
     for (int i = 0; i < ND; i++) o[i] *= alpha;
-#pragma clang loop unroll(disable)
+#pragma clang loop unroll_count(8)
     for (uint32_t j = 0; j < n; j++) {
       const uint32_t kj = k0 + j;
       const float wj = __shfl(w, (int)j);

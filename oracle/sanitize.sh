@@ -36,4 +36,4 @@ LD_PRELOAD="$RT" ASAN_OPTIONS=detect_leaks=0:halt_on_error=1 UBSAN_OPTIONS=halt_
   LLMARIO_HIP_LIB="$OUT/libllmario_hip.so" LLMARIO_ORACLE_LIB="$OUT/liboracle.so" \
   python3 -m pytest -q -p no:cacheprovider tests/test_sched.py tests/test_oracle_attend.py tests/test_oracle_codecs.py \
   tests/test_oracle_pool.py tests/test_oracle_rope.py tests/test_oracle_sched.py tests/test_oracle_snapshot.py \
-  tests/test_oracle_window.py tests/test_golden.py tests/test_native_abi.py tests/test_plan.py tests/test_plan_units.py -m "not gpu"
+  tests/test_oracle_window.py tests/test_golden.py tests/test_native_abi.py tests/test_plan.py tests/test_plan_units.py tests/test_plan_scored.py -m "not gpu"
