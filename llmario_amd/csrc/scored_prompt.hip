@@ -53,6 +53,14 @@ struct Shape {
   static constexpr int ROWS_I = Q8 ? 1 : 2;                 // 1 KiB page rows of an item
 };
 
+// The largest of x over a row of 16 lanes.
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));   // rotated by 1, 2, 4, 8
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+}
+
 // One f32 value of key m, dim d of a tile-layout page (K or V) of head base `head`, tile `sub` of the block.
 template <int KVT>
 __device__ inline float page_value(const uint8_t* head, uint32_t sub, uint32_t tile, uint32_t scale, uint32_t tile_s, bool is_v, uint32_t m,
@@ -184,16 +192,12 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       }
     }
   };
-  ids(0);
-  request(0);
-  ids(1);
-
-  // ---- Q of the wave's columns (the B operand of S^T = K Q^T), while the first tile is on its way
-  uint32_t ct[NCB], ch[NCB], clo[NCB], clen[NCB], cpos[NCB];   // a column sees keys clo .. clo + clen - 1 of the unit's
+  // ---- the wave's columns, and their Q on its way; then the first tile; then the rows' ranges, which lie in host memory
+  // (2 us), so that they are waited for last
+  uint32_t ct[NCB], ch[NCB], cpos[NCB];
   bool cv[NCB];
-  float slope[NCB], qscale[NCB];
-  uint32_t lo_max = 0, end_min = ~0u, lo_min = ~0u, end_max = 0;
-  bool any = false;   // some column of the wave sees a key
+  f4 qv[NCB][NC][2];
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
   for (int x = 0; x < NCB; x++) {
     const uint32_t c = w * COLS + 16 * x + hq;
@@ -201,63 +205,48 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
     ct[x] = cv[x] ? (c + c_off) / G : 0;
     ch[x] = cv[x] ? (c + c_off) - ct[x] * G : 0;
     cpos[x] = pos0 + ct[x];
-    clo[x] = (u.window > 0 && cpos[x] + 1 > u.window) ? cpos[x] + 1 - u.window : 0;
-    uint32_t last = cpos[x];
-    if (sc.ranges) {
-      const uint2 r = sc.ranges[row0 + ct[x]];
-      clo[x] = r.x;
-      last = r.y;
-    }
-    last = min(last, (page_end << 4) - 1);
-    clen[x] = clo[x] <= last ? last + 1 - clo[x] : 0;
-    slope[x] = BIAS && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
-    if (cv[x]) {
-      lo_max = max(lo_max, clo[x]);
-      end_min = min(end_min, last);
-      if (clen[x]) {
-        lo_min = min(lo_min, clo[x]);
-        end_max = max(end_max, last);
-        any = true;
-      }
-    }
-  }
+    const float* qrow = q + ((size_t)(row0 + ct[x]) * u.n_head + (size_t)kvh * G + ch[x]) * HD;
 #pragma unroll
-  for (int i = 1; i < 16; i <<= 1) {
-    lo_max = max(lo_max, (uint32_t)__shfl_xor((int)lo_max, i));
-    end_min = min(end_min, (uint32_t)__shfl_xor((int)end_min, i));
-    lo_min = min(lo_min, (uint32_t)__shfl_xor((int)lo_min, i));
-    end_max = max(end_max, (uint32_t)__shfl_xor((int)end_max, i));
+    for (int k = 0; k < NC; k++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) qv[x][k][e] = cv[x] ? *(const f4u*)(qrow + 32 * k + 8 * grp + 4 * e) : f4u{0.f, 0.f, 0.f, 0.f};
   }
-  lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-  end_min = __builtin_amdgcn_readfirstlane(end_min);
-  lo_min = __builtin_amdgcn_readfirstlane(lo_min);     // no column of the wave sees a key outside lo_min .. end_max
-  end_max = __builtin_amdgcn_readfirstlane(end_max);
-  any = __ballot(any) != 0;
+  __builtin_amdgcn_sched_barrier(0);
+  ids(0);
+  request(0);
+  ids(1);
+  __builtin_amdgcn_sched_barrier(0);
+  uint2 range[NCB];   // first and last key
+  float slope[NCB];
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    range[x] = make_uint2((u.window > 0 && cpos[x] + 1 > u.window) ? cpos[x] + 1 - u.window : 0, cpos[x]);
+    if (sc.ranges) range[x] = sc.ranges[row0 + ct[x]];
+    slope[x] = BIAS && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
+  }
+  __builtin_amdgcn_sched_barrier(0);
+
+  // ---- Q as the B operand of S^T = K Q^T: each column times 2^-e to below 1, in two parts
+  float qscale[NCB];
   h8 qp[2][NCB][NC];
 #pragma unroll
   for (int x = 0; x < NCB; x++) {
-    const float* qrow = q + ((size_t)(row0 + ct[x]) * u.n_head + (size_t)kvh * G + ch[x]) * HD;
-    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-    f4 v[NC][2];
     float am = 0.f;
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-#pragma unroll
-      for (int e = 0; e < 2; e++) v[c][e] = cv[x] ? *(const f4u*)(qrow + 32 * c + 8 * grp + 4 * e) : f4u{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(v[c][i >> 2][i & 3]));
-    }
-    const int e = __builtin_amdgcn_frexp_expf(xmax_groups(am));
-    qscale[x] = ldexpf(u.scale_log2, e);
 #pragma unroll
     for (int c = 0; c < NC; c++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float y = ldexpf(v[c][i >> 2][i & 3], -e);
-        const _Float16 hi = (_Float16)y;
-        qp[0][x][c][i] = hi;
-        qp[1][x][c][i] = (_Float16)(y - (float)hi);
-      }
+      for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(qv[x][c][i >> 2][i & 3]));
+    const int e = min(max(__builtin_amdgcn_frexp_expf(xmax_groups(am)), -126), 126);
+    const float mul = ldexpf(1.0f, -e);
+    qscale[x] = ldexpf(u.scale_log2, e);
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) split_pair(qv[x][c][i >> 1][2 * (i & 1)] * mul, qv[x][c][i >> 1][2 * (i & 1) + 1] * mul, hi[i], lo[i]);
+      qp[0][x][c] = __builtin_bit_cast(h8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      qp[1][x][c] = __builtin_bit_cast(h8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    }
   }
 
   // ---- the powers of two of K and V (bf16, q8_0), from the first tile
@@ -289,8 +278,10 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       if (is_k(i)) top[0] = max(top[0], t);
       else top[1] = max(top[1], t);
     }
+    top[0] = row_max(top[0]);
+    top[1] = row_max(top[1]);
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
+    for (int x = 16; x < 64; x <<= 1) {
       top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], x));
       top[1] = max(top[1], (uint32_t)__shfl_xor((int)top[1], x));
     }
@@ -406,6 +397,30 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
     }
   };
   write(0);
+  // ---- the keys the columns see
+  uint32_t clo[NCB], clen[NCB];   // a column sees keys clo .. clo + clen - 1 of the unit's
+  uint32_t lo_max = 0, hi_min = 0, lo_min = 0, end_max = 0;   // (the least of x as the most of ~x)
+  bool any = false;   // some column of the wave sees a key
+#pragma unroll
+  for (int x = 0; x < NCB; x++) {
+    clo[x] = range[x].x;
+    const uint32_t last = min(range[x].y, (page_end << 4) - 1);
+    clen[x] = clo[x] <= last ? last + 1 - clo[x] : 0;
+    if (cv[x]) {
+      lo_max = max(lo_max, clo[x]);
+      hi_min = max(hi_min, ~last);
+      if (clen[x]) {
+        lo_min = max(lo_min, ~clo[x]);
+        end_max = max(end_max, last);
+        any = true;
+      }
+    }
+  }
+  lo_max = __builtin_amdgcn_readfirstlane(row_max(lo_max));
+  const uint32_t end_min = ~(uint32_t)__builtin_amdgcn_readfirstlane(row_max(hi_min));
+  lo_min = ~(uint32_t)__builtin_amdgcn_readfirstlane(row_max(lo_min));     // no column of the wave sees a key outside lo_min .. end_max
+  end_max = __builtin_amdgcn_readfirstlane(row_max(end_max));
+  any = __ballot(any) != 0;
   __syncthreads();
 
   // ---- the walk
@@ -581,7 +596,6 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
                     q + ((size_t)(row0 + tok) * u.n_head + (size_t)kvh * G + head) * HD, row_at(tok, head), slot != NO_SLOT);
     }
   }
-  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
   for (int x = 0; x < NCB; x++) {
     if (!cv[x]) continue;
