@@ -451,22 +451,27 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       f4 s[NCB][2];
 #pragma unroll
       for (int x = 0; x < NCB; x++) s[x][0] = s[x][1] = f4{0.f, 0.f, 0.f, 0.f};
+      // (products into one accumulator wait for each other: both key blocks' between them)
 #pragma unroll
-      for (int c = 0; c < NC; c++)
+      for (int c = 0; c < NC; c++) {
+        h8 kc[2];
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-          const uint8_t* at = st + ((2 * h + kk) * NC + c) * 1024;
-          const h8 kc = *(const h8*)at;
+        for (int kk = 0; kk < 2; kk++) kc[kk] = *(const h8*)(st + ((2 * h + kk) * NC + c) * 1024);
 #pragma unroll
-          for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qp[0][x][c], s[x][kk], 0, 0, 0);
+        for (int p = 0; p < 2; p++)
 #pragma unroll
-          for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qp[1][x][c], s[x][kk], 0, 0, 0);
-          if constexpr (Q8) {
-            const h8 kl = *(const h8*)(at + C::SIDE);
+          for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-            for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qp[0][x][c], s[x][kk], 0, 0, 0);
-          }
+            for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kk], qp[p][x][c], s[x][kk], 0, 0, 0);
+        if constexpr (Q8) {
+#pragma unroll
+          for (int kk = 0; kk < 2; kk++) kc[kk] = *(const h8*)(st + ((2 * h + kk) * NC + c) * 1024 + C::SIDE);
+#pragma unroll
+          for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+            for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kk], qp[0][x][c], s[x][kk], 0, 0, 0);
         }
+      }
       // the first of V's operands on their way before the softmax
       constexpr int VP = 4;
       const uint8_t* const vst = st + C::PARTS * C::SIDE + h * NJ * 1024;
@@ -524,17 +529,25 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
         pl[x] = __builtin_bit_cast(h8, make_uint4(lw[0], lw[1], lw[2], lw[3]));
       }
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        const uint8_t* at = vst + j * 1024;
-        const h8 va = j < VP ? vpre[j < VP ? j : 0] : *(const h8*)at;
+      for (int j0 = 0; j0 < NJ; j0 += 2) {
+        h8 va[2];
 #pragma unroll
-        for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[x], O[x][j], 0, 0, 0);
+        for (int e = 0; e < 2; e++) va[e] = j0 + e < VP ? vpre[j0 + e < VP ? j0 + e : 0] : *(const h8*)(vst + (j0 + e) * 1024);
 #pragma unroll
-        for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[x], O[x][j], 0, 0, 0);
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], ph[x], O[x][j0 + e], 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], pl[x], O[x][j0 + e], 0, 0, 0);
         if constexpr (Q8) {
-          const h8 vl = *(const h8*)(at + C::SIDE);
 #pragma unroll
-          for (int x = 0; x < NCB; x++) O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[x], O[x][j], 0, 0, 0);
+          for (int e = 0; e < 2; e++) va[e] = *(const h8*)(vst + (j0 + e) * 1024 + C::SIDE);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], ph[x], O[x][j0 + e], 0, 0, 0);
         }
       }
     }
