@@ -20,15 +20,19 @@
 // score by 2^-25 of what the first tile's keys score.
 //
 // Per tile: the next tile's pages are requested into registers, the tile in LDS is multiplied, then the registers are
-// expanded into the other LDS buffer and one barrier publishes it.
+// expanded into the other LDS buffer and one barrier publishes it. All 64 keys' scores are formed before their softmax, so
+// that the second half's weights can issue beside the first half's products (32 keys at a time: q8_0 prompts 106.2 us, 104.8
+// so; four prompts of 2,048 370.7 and 365).
 //
 // Q and the weights in two parts are two products per pair (q8_0: three), so half (a third) of a large product's
 // 1,260 TFLOP/s is the ceiling. Measured, us, with the share of the matrix pipe and of VALU issue: four prompts of 2,048
-// tokens whose first halves see each other, 32/8 heads of 128, bf16: 370, 525 TFLOP/s, 39 % and 35 % (the unit launch 627; a
+// tokens whose first halves see each other, 32/8 heads of 128, bf16: 365, 531 TFLOP/s, 39 % and 35 % (the unit launch 627; a
 // third LDS buffer with the next tile's scores issued ahead of this one's softmax 406 .. 421); three of 401 .. 2,047 on
-// q8_0 pages with a cap 104, 25 % and 33 %, and units of uneven lengths; 8,192 packed tokens of 16/4 heads of 64, f16, 45,
-// 19 % and 32 %: 1,024 units of few tiles, most of it their way from the record to the first tile; two of 600 .. 1,100 tokens,
-// 16/4 heads of 256, bf16, window 1,024, cap 50, 51 and the pieces' merge 5.5, 13 % and 21 %, one workgroup to a CU.
+// q8_0 pages with a cap 102, 25 % and 33 %, and units of uneven lengths; 8,192 packed tokens of 16/4 heads of 64, f16, 42,
+// 19 % and 32 %: 1,024 units of few tiles, much of it their way from the record to the first tile; two of 600 .. 1,100 tokens,
+// 16/4 heads of 256, bf16, window 1,024, cap 50, 49 and the pieces' merge 5.5, 13 % and 21 %, one workgroup to a CU. A unit's
+// time outside its walk, 128-wide heads, by the clock: its record from host memory 2.0 us, Q requested and converted 2 .. 3,
+// the first tile's arrival, maxima and expansion 2, the first pass through the walk's code 1.3, its stores 2.
 // Traffic is small beside that (0.4 .. 1.1 TB/s). No LDS bank conflicts on 16-bit pages; q8_0's 8-byte V stores have a few.
 #include "decode_tile.h"
 #include "score.h"
@@ -424,6 +428,7 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
   __syncthreads();
 
   // ---- the walk
+  constexpr int VP = 4;   // V operands of a tile requested before its softmax (none: q8_0 prompts 104.8 -> 107.7 us)
   constexpr float UP = 7.0f;   // weights up to 2^15: more of them in f16's range
   // a column's weights are taken against mref = m - UP, m a score of it that none exceeds by more than 8 (room: how far
   // scores may exceed mref; -inf before its first, while every score is -inf)
@@ -444,68 +449,68 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
       ids(t + 2);
     }
     const uint8_t* st = prompt_lds + (t & 1) * C::STAGE + lane * 16;
+    const uint32_t key0 = (page0 + 4 * t) << 4;
+    if (any && key0 <= end_max && key0 + 63 >= lo_min) {   // uniform over the wave
+      f4 s[NCB][4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t key0 = ((page0 + 4 * t) << 4) + 32 * h;
-      if (!any || key0 > end_max || key0 + 31 < lo_min) continue;   // uniform over the wave
-      f4 s[NCB][2];
+      for (int x = 0; x < NCB; x++)
 #pragma unroll
-      for (int x = 0; x < NCB; x++) s[x][0] = s[x][1] = f4{0.f, 0.f, 0.f, 0.f};
-      // (products into one accumulator wait for each other: both key blocks' between them)
+        for (int kk = 0; kk < 4; kk++) s[x][kk] = f4{0.f, 0.f, 0.f, 0.f};
+      // (products into one accumulator wait for each other: two key blocks' between them)
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        h8 kc[2];
+      for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) kc[kk] = *(const h8*)(st + ((2 * h + kk) * NC + c) * 1024);
+        for (int c = 0; c < NC; c++) {
+          h8 kc[2];
 #pragma unroll
-        for (int p = 0; p < 2; p++)
+          for (int kk = 0; kk < 2; kk++) kc[kk] = *(const h8*)(st + ((2 * h + kk) * NC + c) * 1024);
 #pragma unroll
-          for (int kk = 0; kk < 2; kk++)
+          for (int p = 0; p < 2; p++)
 #pragma unroll
-            for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kk], qp[p][x][c], s[x][kk], 0, 0, 0);
-        if constexpr (Q8) {
+            for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-          for (int kk = 0; kk < 2; kk++) kc[kk] = *(const h8*)(st + ((2 * h + kk) * NC + c) * 1024 + C::SIDE);
+              for (int x = 0; x < NCB; x++) s[x][2 * h + kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kk], qp[p][x][c], s[x][2 * h + kk], 0, 0, 0);
+          if constexpr (Q8) {
 #pragma unroll
-          for (int kk = 0; kk < 2; kk++)
+            for (int kk = 0; kk < 2; kk++) kc[kk] = *(const h8*)(st + ((2 * h + kk) * NC + c) * 1024 + C::SIDE);
 #pragma unroll
-            for (int x = 0; x < NCB; x++) s[x][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kk], qp[0][x][c], s[x][kk], 0, 0, 0);
+            for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+              for (int x = 0; x < NCB; x++) s[x][2 * h + kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[kk], qp[0][x][c], s[x][2 * h + kk], 0, 0, 0);
+          }
         }
-      }
       // the first of V's operands on their way before the softmax
-      constexpr int VP = 4;
-      const uint8_t* const vst = st + C::PARTS * C::SIDE + h * NJ * 1024;
+      const uint8_t* const vst = st + C::PARTS * C::SIDE;
       h8 vpre[VP];
 #pragma unroll
       for (int j = 0; j < VP; j++) vpre[j] = *(const h8*)(vst + j * 1024);
       __builtin_amdgcn_sched_barrier(0);
-      const bool need_mask = key0 + 31 > end_min || key0 < lo_max;
-      h8 ph[NCB], pl[NCB];
+      const bool need_mask = key0 + 63 > end_min || key0 < lo_max;
+      float p[NCB][16];   // scores less the reference mref
 #pragma unroll
       for (int x = 0; x < NCB; x++) {
-        float p[8];   // scores less the reference mref
         if constexpr (CAP) {
 #pragma unroll
-          for (int i = 0; i < 8; i++) p[i] = s[x][i >> 2][i & 3] * qscale[x];
-          cap_scores<8>(p, sc.cap_log2);
+          for (int i = 0; i < 16; i++) p[x][i] = s[x][i >> 2][i & 3] * qscale[x];
+          cap_scores<16>(p[x], sc.cap_log2);
 #pragma unroll
-          for (int i = 0; i < 8; i++) p[i] -= mref[x];
+          for (int i = 0; i < 16; i++) p[x][i] -= mref[x];
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; i++) p[i] = fmaf(s[x][i >> 2][i & 3], qscale[x], -mref[x]);
+          for (int i = 0; i < 16; i++) p[x][i] = fmaf(s[x][i >> 2][i & 3], qscale[x], -mref[x]);
         }
-        if constexpr (BIAS) bias_scores<8>(p, slope[x], (float)(int)(key0 + 4 * grp - cpos[x]), [](int i) { return (float)(16 * (i >> 2) + (i & 3)); });
+        if constexpr (BIAS) bias_scores<16>(p[x], slope[x], (float)(int)(key0 + 4 * grp - cpos[x]), [](int i) { return (float)(16 * (i >> 2) + (i & 3)); });
         if (need_mask) {
           const uint32_t at = key0 + 4 * grp - clo[x];   // (keys before clo wrap round)
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            p[i] = at + 16 * (i >> 2) + (i & 3) < clen[x] ? p[i] : -INFINITY;
-            asm volatile("" : "+v"(p[i]));   // not ahead of the test
+          for (int i = 0; i < 16; i++) {
+            p[x][i] = at + 16 * (i >> 2) + (i & 3) < clen[x] ? p[x][i] : -INFINITY;
+            asm volatile("" : "+v"(p[x][i]));   // not ahead of the test
           }
         }
-        float lm = p[0];
+        float lm = p[x][0];
 #pragma unroll
-        for (int i = 1; i < 8; i++) lm = fmaxf(lm, p[i]);
+        for (int i = 1; i < 16; i++) lm = fmaxf(lm, p[x][i]);
         if (__ballot(lm > room[x])) {   // some column's largest score is 8 past its m, or its first
           const float tm = xmax_groups(lm) + mref[x];
           if (tm - mref[x] > room[x]) {
@@ -514,42 +519,57 @@ void scored_prompt_kernel(PageGeom g, UnitGeom u, ScoreGeom sc, const PromptItem
 #pragma unroll
             for (int j = 0; j < NJ; j++) O[x][j] *= alpha;
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] -= nref - mref[x];
+            for (int i = 0; i < 16; i++) p[x][i] -= nref - mref[x];
             mref[x] = nref;
             room[x] = UP + 8.0f;
           }
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = exp2_fast(p[i]);
-        lsum[x] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        uint32_t hw[4], lw[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) split_pair(p[2 * i], p[2 * i + 1], hw[i], lw[i]);
-        ph[x] = __builtin_bit_cast(h8, make_uint4(hw[0], hw[1], hw[2], hw[3]));
-        pl[x] = __builtin_bit_cast(h8, make_uint4(lw[0], lw[1], lw[2], lw[3]));
       }
+      // weights of half h; those of the second beside the products of the first
+      h8 ph[2][NCB], pl[2][NCB];
+      auto weights = [&](int h) {
 #pragma unroll
-      for (int j0 = 0; j0 < NJ; j0 += 2) {
-        h8 va[2];
+        for (int x = 0; x < NCB; x++) {
+          float* e = p[x] + 8 * h;
 #pragma unroll
-        for (int e = 0; e < 2; e++) va[e] = j0 + e < VP ? vpre[j0 + e < VP ? j0 + e : 0] : *(const h8*)(vst + (j0 + e) * 1024);
+          for (int i = 0; i < 8; i++) e[i] = exp2_fast(e[i]);
+          lsum[x] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+          uint32_t hw[4], lw[4];
 #pragma unroll
-        for (int e = 0; e < 2; e++)
+          for (int i = 0; i < 4; i++) split_pair(e[2 * i], e[2 * i + 1], hw[i], lw[i]);
+          ph[h][x] = __builtin_bit_cast(h8, make_uint4(hw[0], hw[1], hw[2], hw[3]));
+          pl[h][x] = __builtin_bit_cast(h8, make_uint4(lw[0], lw[1], lw[2], lw[3]));
+        }
+      };
+      auto products = [&](int h) {
+        const uint8_t* const vh = vst + h * NJ * 1024;
 #pragma unroll
-          for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], ph[x], O[x][j0 + e], 0, 0, 0);
+        for (int j0 = 0; j0 < NJ; j0 += 2) {
+          h8 va[2];
 #pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-          for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], pl[x], O[x][j0 + e], 0, 0, 0);
-        if constexpr (Q8) {
-#pragma unroll
-          for (int e = 0; e < 2; e++) va[e] = *(const h8*)(vst + (j0 + e) * 1024 + C::SIDE);
+          for (int e = 0; e < 2; e++) va[e] = h == 0 && j0 + e < VP ? vpre[j0 + e < VP ? j0 + e : 0] : *(const h8*)(vh + (j0 + e) * 1024);
 #pragma unroll
           for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], ph[x], O[x][j0 + e], 0, 0, 0);
+            for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], ph[h][x], O[x][j0 + e], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], pl[h][x], O[x][j0 + e], 0, 0, 0);
+          if constexpr (Q8) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) va[e] = *(const h8*)(vh + (j0 + e) * 1024 + C::SIDE);
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+              for (int x = 0; x < NCB; x++) O[x][j0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], ph[h][x], O[x][j0 + e], 0, 0, 0);
+          }
         }
-      }
+      };
+      weights(0);
+      products(0);
+      weights(1);
+      products(1);
     }
     if (t + 1 < n_tiles) write((t + 1) & 1);
     __syncthreads();
