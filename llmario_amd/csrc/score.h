@@ -7,6 +7,14 @@ namespace lmh {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// The largest of x over a row of 16 lanes.
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));   // rotated by 1, 2, 4, 8
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+}
+
 // cap * tanh(u) of N scores, u = score / cap and cap in the log2 domain (cap * log2(e)). While every |u| of the wave
 // is at most 3/4, by a polynomial: tanh(u) = u + u^3 P(u^2), P of degree 4 fitted to the least largest error relative to
 // tanh(u), 3.2e-8 of it (2.4 * 2^-24 as evaluated in f32, 0.7 * 2^-24 in the mean): nine multiply-adds. Caps are far above

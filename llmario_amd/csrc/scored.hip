@@ -10,7 +10,7 @@
 // 32/8 heads of 128, f16, cap 50: 40 us, 5.8 TB/s of the 6.9 a plain read reaches, VALU 15 % and matrix pipe 7 % of its
 // time; 8 on 32,768 q8_0 keys with slopes 99 .. 112 us, 5.2 .. 5.8 TB/s, VALU 44 % (codes to f16, a unit's scales).
 // Smaller ones are bound by the chain of a wave's steps and the widest unit's share of a workgroup: 48 sequences of
-// packed documents, 40/8 heads, bf16, 127 MB: 31.7 us, one wave per SIMD; 8 rows beside 120 of a prompt, 32 heads of 80:
+// packed documents, 40/8 heads, bf16, 127 MB: 31 us, one wave per SIMD; 8 rows beside 120 of a prompt, 32 heads of 80:
 // 26 us, 3.4 TB/s; one f32 row of 256 keys 10 us, a launch and five dependent round trips. Cut units' merge: 4.1 us.
 #include "unit_wave.h"
 

@@ -57,14 +57,6 @@ struct Shape {
   static constexpr int ROWS_I = Q8 ? 1 : 2;                 // 1 KiB page rows of an item
 };
 
-// The largest of x over a row of 16 lanes.
-__device__ __forceinline__ uint32_t row_max(uint32_t x) {
-  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));   // rotated by 1, 2, 4, 8
-  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
-  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
-  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
-}
-
 // One f32 value of key m, dim d of a tile-layout page (K or V) of head base `head`, tile `sub` of the block.
 template <int KVT>
 __device__ inline float page_value(const uint8_t* head, uint32_t sub, uint32_t tile, uint32_t scale, uint32_t tile_s, bool is_v, uint32_t m,

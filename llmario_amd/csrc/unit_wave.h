@@ -128,31 +128,12 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
         slope[x] = sc.slopes && cv[x] ? sc.slopes[kvh * G + ch[x]] * LOG2E : 0.f;
       }
     }
-    if (SC && sc.ranges) {
-      lo_max = 0;
-      end_min = ~0u;
-#pragma unroll
-      for (int x = 0; x < NB; x++) {
-        const uint2 r = sc.ranges[row0 + ct[x]];
-        clo[x] = r.x;
-        cend[x] = r.y;
-        if (cv[x]) {
-          lo_max = max(lo_max, r.x);
-          end_min = min(end_min, r.y);
-        }
-      }
-#pragma unroll
-      for (int i = 1; i < 16; i <<= 1) {
-        lo_max = max(lo_max, (uint32_t)__shfl_xor((int)lo_max, i));
-        end_min = min(end_min, (uint32_t)__shfl_xor((int)end_min, i));
-      }
-      lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-      end_min = __builtin_amdgcn_readfirstlane(end_min);
-    } else {
+    {
       const uint32_t pos_last = pos0 + (c_off + n_col - 1) / G;
       lo_max = (u.window > 0 && pos_last + 1 > u.window) ? pos_last + 1 - u.window : 0;
       end_min = pos0;
     }
+    uint2 range[NB];   // the rows' own ranges, in host memory (2 us): requested behind K, V and Q, waited for after Q's conversion
 
     // ---- page addresses: block ids through scalar loads (the table does not change while the
     // kernel runs), the first step's from the record
@@ -267,6 +248,10 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
           const uint32_t d = 16 * c + 4 * grp;
           qf[x][c] = cv[x] && d < hd ? *(const f4u*)(qrow + d) : f4u{0.f, 0.f, 0.f, 0.f};
         }
+        if (SC && x == 0 && sc.ranges) {
+#pragma unroll
+          for (int y = 0; y < NB; y++) range[y] = sc.ranges[row0 + ct[y]];
+        }
       } else {
         f4 raw[NC][2];
 #pragma unroll
@@ -275,6 +260,10 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
           const bool on = cv[x] && (!ROWS || d < hd);
           raw[c][0] = on ? *(const f4u*)(qrow + d) : f4u{0.f, 0.f, 0.f, 0.f};
           raw[c][1] = on ? *(const f4u*)(qrow + d + 4) : f4u{0.f, 0.f, 0.f, 0.f};
+        }
+        if (SC && x == 0 && sc.ranges) {
+#pragma unroll
+          for (int y = 0; y < NB; y++) range[y] = sc.ranges[row0 + ct[y]];
         }
         if constexpr (F == FR_F16 || (SC && !BF)) {   // (shaped scores: f16 parts of a Q far from 1 too)
           float am = 0.f;
@@ -317,6 +306,22 @@ __device__ __forceinline__ void unit_wave(const PageGeom& g, const UnitGeom& u, 
           }
         }
       }
+    }
+
+    if (SC && sc.ranges) {
+      uint32_t last_min = 0;   // (as the most of ~last)
+      lo_max = 0;
+#pragma unroll
+      for (int x = 0; x < NB; x++) {
+        clo[x] = range[x].x;
+        cend[x] = range[x].y;
+        if (cv[x]) {
+          lo_max = max(lo_max, range[x].x);
+          last_min = max(last_min, ~range[x].y);
+        }
+      }
+      lo_max = __builtin_amdgcn_readfirstlane(row_max(lo_max));
+      end_min = ~(uint32_t)__builtin_amdgcn_readfirstlane(row_max(last_min));
     }
 
     // pup, `checked`: as decode_item's (q8_0: weight x V scale in f16 range; a product that
