@@ -103,14 +103,18 @@ __device__ __forceinline__ void redo(const PageGeom& g, const UnitGeom& u, const
     l = l * alpha + sum;
     m = mn;
     for (int i = 0; i < ND; i++) o[i] *= alpha;
-#pragma clang loop unroll_count(8)
-    for (uint32_t j = 0; j < n; j++) {
-      const uint32_t kj = k0 + j;
-      const float wj = __shfl(w, (int)j);
-      const uint8_t* vh = g.pool + (size_t)(uint32_t)tab[kj >> g.bt_shift] * g.block_bytes + g.v_off + (size_t)kvh * g.v_head;
-      for (int i = 0; i < ND; i++)
-        o[i] = fmaf(wj, page_value<KVT>(vh, (kj & bt_mask) >> 4, g.v_tile, g.v_scale, g.v_tile_s, true, kj & 15u, lane + 64 * i, HD), o[i]);
-    }
+#pragma clang loop unroll(disable)
+    for (uint32_t j0 = 0; j0 < n; j0 += 8)
+#pragma unroll
+      for (uint32_t e = 0; e < 8; e++) {
+        const uint32_t kj = min(k0 + j0 + e, end - 1);   // (past the last: read again, not added)
+        const float wj = __shfl(w, (int)(j0 + e));
+        const uint8_t* vh = g.pool + (size_t)(uint32_t)tab[kj >> g.bt_shift] * g.block_bytes + g.v_off + (size_t)kvh * g.v_head;
+        for (int i = 0; i < ND; i++) {
+          const float v = page_value<KVT>(vh, (kj & bt_mask) >> 4, g.v_tile, g.v_scale, g.v_tile_s, true, kj & 15u, lane + 64 * i, HD);
+          o[i] = j0 + e < n ? fmaf(wj, v, o[i]) : o[i];
+        }
+      }
   }
   const float mul = partial ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
   for (int i = 0; i < ND; i++) out[lane + 64 * i] = o[i] * mul;
